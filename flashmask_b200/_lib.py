@@ -43,6 +43,42 @@ class AttnArgs(C.Structure):
     ]
 
 
+class NormRotaryArgs(C.Structure):
+    """Mirror of ``fm_norm_rotary_args``."""
+    _fields_ = [
+        ("B", C.c_int32), ("S", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("d", C.c_int32), ("rot", C.c_int32),
+        ("dtype", C.c_int32), ("interleaved", C.c_int32), ("weight_f32", C.c_int32), ("table", C.c_int32),
+        ("positions_64", C.c_int32), ("eps", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+        ("cos", C.c_void_p), ("sin", C.c_void_p), ("positions", C.c_void_p), ("positions_stride", C.c_int64),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("d_q", C.c_void_p), ("d_k", C.c_void_p),
+        ("dq_weight", C.c_void_p), ("dk_weight", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("q_stride", I64x3), ("k_stride", I64x3), ("qo_stride", I64x3), ("ko_stride", I64x3),
+        ("dq_stride", I64x3), ("dk_stride", I64x3),
+    ]
+
+
+class KvCache(C.Structure):
+    """Mirror of ``fm_kv_cache``."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_int32), ("page_size", C.c_int32), ("Hkv", C.c_int32), ("d", C.c_int32),
+                ("dv", C.c_int32), ("dtype", C.c_int32)]
+
+
+class KvArgs(C.Structure):
+    """Mirror of ``fm_kv_args``."""
+    _fields_ = [
+        ("B", C.c_int32), ("S", C.c_int32), ("Hq", C.c_int32), ("dtype", C.c_int32), ("max_pages", C.c_int32),
+        ("causal", C.c_int32), ("window", C.c_int32), ("softmax_scale", C.c_float), ("table_stride", C.c_int64),
+        ("page_table", C.c_void_p), ("seqlens", C.c_void_p), ("start", C.c_void_p), ("lengths", C.c_void_p),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("sink", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("q_stride", I64x3), ("k_stride", I64x3), ("v_stride", I64x3),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/flashmask_b200.h declares
 SIGNATURES = {
     "fm_version": (C.c_char_p, []),
@@ -86,6 +122,15 @@ SIGNATURES = {
     "fm_cp_cast": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p]),
     "fm_cp_reduce_partials": (C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_void_p, C.c_int64, C.c_int,
                                         C.c_void_p]),
+    "fm_norm_rotary_fwd": (C.c_int, [C.POINTER(NormRotaryArgs), C.c_void_p]),
+    "fm_norm_rotary_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(NormRotaryArgs)]),
+    "fm_norm_rotary_bwd": (C.c_int, [C.POINTER(NormRotaryArgs), C.c_void_p]),
+    "fm_kv_locate": (C.c_int64, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_int, C.c_int, C.c_int64, C.c_int]),
+    "fm_kv_write": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_void_p]),
+    "fm_kv_read": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_void_p]),
+    "fm_kv_attention_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvArgs)]),
+    "fm_kv_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_void_p]),
+    "fm_kv_bounds": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 
 _lib = None

@@ -5,9 +5,9 @@
 Every ``csrc/*.cu`` is compiled to an object under ``build/`` (in parallel,
 skipped when the object is newer than all sources and headers) and linked into
 ``flashmask_b200/libflashmask_b200.so``.  The host C++ solver sources
-(``csrc/*.cpp``) go through the same nvcc invocation.  ``csrc/torch/fm_torch.cpp``,
-the native host path of the operator, is compiled against torch into
-``flashmask_b200/_host.so`` and finds the library beside itself.
+(``csrc/*.cpp``) go through the same nvcc invocation.  ``csrc/torch/*.cpp``,
+the native host path of the operators, is compiled against torch and linked into
+``flashmask_b200/_host.so``, which finds the library beside itself.
 """
 from __future__ import annotations
 
@@ -23,7 +23,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "libflashmask_b200.so")
-HOST_SRC = os.path.join(CSRC, "torch", "fm_torch.cpp")
+HOST_DIR = os.path.join(CSRC, "torch")
 HOST_OUT = os.path.join(PKG, "_host.so")
 OBJ = os.path.join(ROOT, "build", "obj")
 
@@ -55,20 +55,25 @@ def headers():
             glob.glob(os.path.join(ROOT, "include", "*.h")) + [os.path.abspath(__file__)])
 
 
-def _host_command():
-    """g++ invocation of the native host path (no device code, no pybind beyond torch's own)."""
+def _host_commands():
+    """g++ invocations of the native host path (no device code, no pybind beyond torch's own): (source, object,
+    command) of every source, and the link."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    gxx = shutil.which("g++") or "g++"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for d in ce.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include"),
                                    os.path.join(ROOT, "include")]:
-        cmd += ["-isystem", d]
-    return cmd + [HOST_SRC, "-o", HOST_OUT, f"-L{lib}", f"-L{PKG}", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-                  "-lc10", "-lc10_cuda", "-l:libflashmask_b200.so", "-Wl,-rpath,$ORIGIN"]
+        flags += ["-isystem", d]
+    srcs = sorted(glob.glob(os.path.join(HOST_DIR, "*.cpp")))
+    objs = [os.path.join(OBJ, os.path.basename(s) + ".host.o") for s in srcs]
+    link = [gxx, "-shared"] + objs + ["-o", HOST_OUT, f"-L{lib}", f"-L{PKG}", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+                                      "-lc10", "-lc10_cuda", "-l:libflashmask_b200.so", "-Wl,-rpath,$ORIGIN"]
+    return [(s, o, [gxx] + flags + ["-c", s, "-o", o]) for s, o in zip(srcs, objs)], link
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -106,13 +111,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
-    hdr = os.path.join(ROOT, "include", "flashmask_b200.h")
-    if force or _stale(HOST_OUT, [HOST_SRC, hdr, os.path.abspath(__file__)]):
-        r = subprocess.run(_host_command(), capture_output=True, text=True)
-        if verbose or r.returncode:
-            sys.stderr.write(r.stdout + r.stderr)
+    deps = [os.path.join(ROOT, "include", "flashmask_b200.h"), os.path.abspath(__file__)] + glob.glob(os.path.join(HOST_DIR, "*.h"))
+    hosts, link = _host_commands()
+    stale = [(s, cmd) for s, o, cmd in hosts if force or _stale(o, [s] + deps)]
+    with cf.ThreadPoolExecutor(max_workers=max(1, len(stale))) as ex:
+        for s, r in ex.map(run, stale):
+            if verbose or r.returncode:
+                sys.stderr.write(f"--- {os.path.basename(s)}\n{r.stdout}{r.stderr}\n")
+            if r.returncode:
+                raise RuntimeError(f"g++ failed on {s}")
+    if stale or force or _stale(HOST_OUT, [o for _, o, _ in hosts]):
+        r = subprocess.run(link, capture_output=True, text=True)
         if r.returncode:
-            raise RuntimeError(f"g++ failed on {HOST_SRC}")
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("link of the native host failed")
     return OUT
 
 

@@ -1,0 +1,327 @@
+// Writing 16-bit keys and values into the 8-bit paged cache, and reading them back.
+#include <algorithm>
+
+#include "fm_kv_cache.cuh"
+
+namespace fm {
+
+struct KvWriteParams {
+  KvGeom g;
+  uint8_t* pay[2]; float* scale[2];
+  const uint16_t* src[2];
+  int64_t stride[2][3];
+  int width[2];
+  const int32_t* table; const int32_t* start; const int32_t* lengths;
+  int B, S;
+};
+
+// One CTA = one page of one kv head, K or V (blockIdx.y = 2 * head + which), of the pages that the new tokens of sequence
+// blockIdx.z reach.  It reads its tokens once, keeps them in registers while the CTA finds the largest magnitude, and
+// writes one byte for every two that it read.  Bound by HBM: 3 bytes a value.
+// A page that held tokens before (the write starts inside it) keeps its scale or grows it; where it grows, the payload
+// of the earlier tokens is rounded on the new grid.  Slots behind the last new token are left as they are.
+// VEC = units of 8 values that a thread holds.
+template <bool IS_BF16, bool INT8, int VEC>
+__global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteParams p) {
+  __shared__ float s_max[8];
+  __shared__ int s_nan[8];
+  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, P = 1 << p.g.page_log2;
+  const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
+  const int start = p.start[b];
+  const int skip = start < 0 ? -start : 0;                       // rows before position 0 are not written
+  if (n <= skip || start > INT_MAX - p.S) return;
+  const int first = max(start, 0), last = start + n - 1;         // positions
+  const int base = ((first >> p.g.page_log2) + (int)blockIdx.x) << p.g.page_log2;
+  if (base > last || base < 0) return;
+  const int page = kv_page(p.g, p.table + b * p.g.table_stride, base);
+  if (page < 0) return;
+  const int w = p.width[which], upr = w >> 3;                     // units of 8 values in a row
+  const int lo = max(first - base, 0), hi = min(last - base + 1, P);       // slots [lo, hi) are new
+  uint8_t* pay = p.pay[which] + ((size_t)page * p.g.Hkv + h) * P * w;
+  float* scale = p.scale[which] + (size_t)page * p.g.Hkv + h;
+  const uint16_t* src = p.src[which] + b * p.stride[which][0] + h * p.stride[which][2];
+  const int64_t ss = p.stride[which][1];
+  const float old = lo > 0 ? *scale : 0.f;
+  const int n_units = (hi - lo) * upr;
+  uint4 x[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const int u = threadIdx.x + i * blockDim.x;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (u < n_units) {
+      const int row = u / upr;
+      x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)(base + lo + row - start) * ss + (u - row * upr) * 8));
+    }
+  }
+  float amax = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float2 f = unpack2<IS_BF16>(v[c]);
+      const float a = fabsf(f.x), d = fabsf(f.y);
+      // (a value that is no number does not set the scale)
+      if (a <= 3.4e38f) amax = fmaxf(amax, a); else bad = true;
+      if (d <= 3.4e38f) amax = fmaxf(amax, d); else bad = true;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  bad = __any_sync(0xffffffffu, bad);
+  const int warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) { s_max[warp] = amax; s_nan[warp] = bad; }
+  __syncthreads();
+  for (int i = 0; i < n_warps; ++i) { amax = fmaxf(amax, s_max[i]); bad |= s_nan[i] != 0; }
+  int e = cache_exponent<INT8>(amax);
+  const bool old_nan = INT8 && lo > 0 && !(old > 0.f);           // a NaN scale stays until the page is started again
+  const int e_old = (int)(__float_as_uint(old) >> 23 & 0xff) - 127;
+  if (lo > 0 && !old_nan) e = max(e, min(max(e_old, kCacheMinExp), kCacheMaxExp<INT8>));
+  const float inv = exp2_int(-e);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const int u = threadIdx.x + i * blockDim.x;
+    if (u < n_units) {
+      const int row = u / upr;
+      const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint32_t r[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float2 f = unpack2<IS_BF16>(v[c]);
+        // what is no number has no payload: NaN in e4m3, 0 in int8, where the scale says it
+        const float none = INT8 ? 0.f : __uint_as_float(0x7fffffffu);
+        if (!(fabsf(f.x) <= 3.4e38f)) f.x = none;
+        if (!(fabsf(f.y) <= 3.4e38f)) f.y = none;
+        r[c] = to_payload2<INT8>(f.x * inv, f.y * inv);
+      }
+      *reinterpret_cast<uint2*>(pay + (size_t)(lo + row) * w + (u - row * upr) * 8) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+    }
+  }
+  if (lo > 0 && !old_nan && e > e_old) {
+    const float f = exp2_int(max(e_old - e, -126));
+    for (int u = threadIdx.x; u < lo * upr; u += blockDim.x) {
+      uint2* at = reinterpret_cast<uint2*>(pay) + u;
+      uint2 v = *at;
+      float a[4];
+      payload_f32<INT8>(v.x, a);
+      v.x = to_payload2<INT8>(a[0] * f, a[1] * f) | to_payload2<INT8>(a[2] * f, a[3] * f) << 16;
+      payload_f32<INT8>(v.y, a);
+      v.y = to_payload2<INT8>(a[0] * f, a[1] * f) | to_payload2<INT8>(a[2] * f, a[3] * f) << 16;
+      *at = v;
+    }
+  }
+  // every thread has read the old scale (the barrier above), so it can go
+  if (threadIdx.x == 0) *scale = INT8 && (bad || old_nan) ? __uint_as_float(0x7fffffffu) : exp2_int(e);
+}
+
+struct KvReadParams {
+  KvGeom g;
+  const uint8_t* pay[2]; const float* scale[2];
+  uint16_t* dst[2];
+  int width[2];
+  const int32_t* table; const int32_t* start; const int32_t* seqlens;
+  int B, S;
+};
+
+// dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  A thread takes 8 values at a time (8
+// bytes in, 16 out, neighbouring threads neighbouring units of the output) and has READ_ILP of them in flight, since each
+// is behind a page number and next to a scale.  Bound by HBM: 3 bytes a value.
+constexpr int READ_ILP = 4;
+template <bool IS_BF16, bool INT8>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
+  const int b = blockIdx.y, which = blockIdx.z, w = p.width[which], upr = w >> 3, P = 1 << p.g.page_log2;
+  const uint32_t per_row = p.g.Hkv * upr;
+  const int64_t n_units = (int64_t)p.S * per_row;
+  const int start = p.start[b], len = kv_len(p.g, p.seqlens[b]);
+  const int32_t* row = p.table + b * p.g.table_stride;
+  uint16_t* dst = p.dst[which] + (size_t)b * p.S * p.g.Hkv * w;
+  const int64_t u0 = (int64_t)blockIdx.x * (256 * READ_ILP) + threadIdx.x;
+  uint2 v[READ_ILP];
+  float sc[READ_ILP];
+#pragma unroll
+  for (int i = 0; i < READ_ILP; ++i) {
+    const int64_t u = u0 + i * 256;
+    v[i] = make_uint2(0, 0);
+    sc[i] = 0.f;
+    if (u < n_units) {
+      const int s = (int)(u / per_row);
+      const uint32_t r = (uint32_t)(u - (int64_t)s * per_row), h = r / upr, c = r - h * upr;
+      const int64_t pos = (int64_t)start + s;
+      const int page = pos >= 0 && pos < len ? kv_page(p.g, row, (int)pos) : -1;
+      if (page >= 0) {
+        const size_t ph = (size_t)page * p.g.Hkv + h;
+        v[i] = __ldcs(reinterpret_cast<const uint2*>(p.pay[which] + (ph * P + (pos & (P - 1))) * w + c * 8));
+        sc[i] = __ldg(p.scale[which] + ph);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < READ_ILP; ++i) {
+    const int64_t u = u0 + i * 256;
+    if (u >= n_units) break;
+    float a[4], c[4];
+    payload_f32<INT8>(v[i].x, a);
+    payload_f32<INT8>(v[i].y, c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] *= sc[i]; c[j] *= sc[i];
+      // the 8-bit grid reaches a little beyond fp16; NaN passes
+      if (!IS_BF16) { if (fabsf(a[j]) > 65504.f) a[j] = copysignf(65504.f, a[j]); if (fabsf(c[j]) > 65504.f) c[j] = copysignf(65504.f, c[j]); }
+    }
+    *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(pack2<IS_BF16>(a[0], a[1]), pack2<IS_BF16>(a[2], a[3]),
+                                                         pack2<IS_BF16>(c[0], c[1]), pack2<IS_BF16>(c[2], c[3]));
+  }
+}
+
+// Column bounds that make a dense causal forward over the read-back tokens see what the cache's rows see.  Column c
+// of sequence b holds position shift_b + c.  With `n` real query rows (of Sq) and rows counted from the first, position
+// p is hidden from row i on: i >= n (no query), i >= p - p0 + window (out of the window), and everywhere when it is no
+// token.  Causal: lower bound alone.
+struct KvBoundsParams {
+  KvGeom g;
+  const int32_t* seqlens; const int32_t* lengths; const int32_t* table;
+  int32_t* shift; int32_t* bounds;
+  int B, Sq, cols, causal, window;
+};
+__global__ void __launch_bounds__(256) kv_bounds_kernel(const KvBoundsParams p) {
+  const int b = blockIdx.y;
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int len = kv_len(p.g, p.seqlens[b]);
+  const int n = p.lengths ? min(max(p.lengths[b], 0), p.Sq) : p.Sq;
+  // the first row stands at len - n and, bottom-right aligned, sees the columns up to cols - Sq
+  const int shift = len - n - (p.cols - p.Sq);
+  if (c == 0) p.shift[b] = shift;
+  if (c >= p.cols) return;
+  const int pos = shift + c;
+  int end = 0;
+  if (pos >= 0 && pos < len && kv_page(p.g, p.table + b * p.g.table_stride, pos) >= 0) {
+    end = n;
+    if (p.window > 0) end = (int)min((int64_t)end, (int64_t)pos - (len - n) + p.window);
+  }
+  end = max(end, 0);
+  if (p.causal) p.bounds[(int64_t)b * p.cols + c] = end;
+  else reinterpret_cast<int2*>(p.bounds)[(int64_t)b * p.cols + c] = make_int2(end, 0);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+static int page_log2_of(int page_size) {
+  for (int l = 4; l <= 7; ++l)
+    if (page_size == 1 << l) return l;
+  return -1;
+}
+
+int kv_geometry(const fm_kv_cache* c, const fm_kv_args* a, KvGeom* g) {
+  FM_REQUIRE(c && a, FM_ERR_INVALID_ARGUMENT, "kv cache: NULL argument");
+  FM_REQUIRE(c->k && c->v && c->k_scale && c->v_scale, FM_ERR_INVALID_ARGUMENT, "kv cache: payload or scale is NULL");
+  FM_REQUIRE(c->dtype == FM_CACHE_E4M3 || c->dtype == FM_CACHE_INT8, FM_ERR_INVALID_ARGUMENT, "kv cache: unknown payload type %d", c->dtype);
+  FM_REQUIRE(a->dtype == FM_DTYPE_BF16 || a->dtype == FM_DTYPE_FP16, FM_ERR_INVALID_ARGUMENT, "kv cache: unknown dtype %d", a->dtype);
+  FM_REQUIRE(c->num_pages > 0 && c->Hkv > 0, FM_ERR_INVALID_ARGUMENT, "kv cache: num_pages=%d, Hkv=%d", c->num_pages, c->Hkv);
+  FM_REQUIRE(page_log2_of(c->page_size) > 0, FM_ERR_UNSUPPORTED, "kv cache: page_size %d is not 16, 32, 64 or 128", c->page_size);
+  FM_REQUIRE(c->d > 0 && c->dv > 0 && c->d % 16 == 0 && c->dv % 16 == 0, FM_ERR_UNSUPPORTED,
+             "kv cache: head dims %d / %d are not multiples of 16", c->d, c->dv);
+  FM_REQUIRE((c->d <= 128 && c->dv <= 128) || (c->d == 192 && c->dv == 128) || (c->d == 256 && c->dv == 256), FM_ERR_UNSUPPORTED,
+             "kv cache: head dims %d / %d are not served (<= 128, 192 / 128, 256 / 256)", c->d, c->dv);
+  FM_REQUIRE(((uintptr_t)c->k & 15) == 0 && ((uintptr_t)c->v & 15) == 0, FM_ERR_INVALID_ARGUMENT, "kv cache: payload is not 16-byte aligned");
+  FM_REQUIRE(a->B >= 0 && a->S >= 0 && a->max_pages >= 0, FM_ERR_INVALID_ARGUMENT, "kv cache: negative size");
+  FM_REQUIRE(a->B <= 65535 && c->Hkv <= 32767, FM_ERR_UNSUPPORTED, "kv cache: more than 65535 sequences or 32767 heads");
+  FM_REQUIRE((int64_t)a->max_pages * c->page_size < INT_MAX - 65536, FM_ERR_UNSUPPORTED, "kv cache: a page table of more than 2^31 positions");
+  FM_REQUIRE(a->page_table || a->B == 0 || a->max_pages == 0, FM_ERR_INVALID_ARGUMENT, "kv cache: page_table is NULL");
+  FM_REQUIRE(a->table_stride >= a->max_pages || a->B <= 1, FM_ERR_INVALID_ARGUMENT, "kv cache: table_stride below max_pages");
+  g->num_pages = c->num_pages; g->page_log2 = page_log2_of(c->page_size); g->Hkv = c->Hkv;
+  g->max_pages = a->max_pages; g->table_stride = a->table_stride;
+  return FM_OK;
+}
+
+template <bool IS_BF16, bool INT8>
+static int launch_write(const KvWriteParams& p, int page_size, int width_max, cudaStream_t s) {
+  const int units = page_size * width_max / 8;                     // <= 4096
+  const int threads = std::min(256, (units + 31) / 32 * 32);
+  const int64_t pages = ((int64_t)p.S + page_size - 2) / page_size + 1;      // wherever the first token falls
+  const dim3 grid((unsigned)pages, 2 * p.g.Hkv, p.B);
+  const int vec = (units + threads - 1) / threads;
+#define FM_KV_WRITE(N) if (vec <= N) { kv_write_kernel<IS_BF16, INT8, N><<<grid, threads, 0, s>>>(p); }
+  FM_KV_WRITE(1) else FM_KV_WRITE(2) else FM_KV_WRITE(4) else FM_KV_WRITE(8) else FM_KV_WRITE(16)
+#undef FM_KV_WRITE
+  count_launches(1);
+  FM_CUDA_TRY(cudaGetLastError());
+  return FM_OK;
+}
+
+}  // namespace fm
+
+using namespace fm;
+
+extern "C" FM_API int64_t fm_kv_locate(const fm_kv_cache* c, const fm_kv_args* a, int b, int head, int64_t pos, int value) {
+  KvGeom g;
+  if (kv_geometry(c, a, &g) != FM_OK || b < 0 || b >= a->B || head < 0 || head >= c->Hkv || pos < INT_MIN || pos > INT_MAX) return -1;
+  const int page = kv_page(g, a->page_table + (int64_t)b * g.table_stride, (int)pos);
+  if (page < 0) return -1;
+  return (((int64_t)page * c->Hkv + head) * c->page_size + (pos & (c->page_size - 1))) * (value ? c->dv : c->d);
+}
+
+extern "C" FM_API int fm_kv_write(const fm_kv_cache* c, const fm_kv_args* a, void* stream) {
+  KvWriteParams p;
+  const int rc = kv_geometry(c, a, &p.g);
+  if (rc) return rc;
+  if (a->B == 0 || a->S == 0 || a->max_pages == 0) return FM_OK;
+  FM_REQUIRE(a->k && a->v && a->start, FM_ERR_INVALID_ARGUMENT, "fm_kv_write: key, value or start is NULL");
+  FM_REQUIRE(((uintptr_t)a->k & 15) == 0 && ((uintptr_t)a->v & 15) == 0, FM_ERR_INVALID_ARGUMENT, "fm_kv_write: key or value is not 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    FM_REQUIRE(a->k_stride[i] % 8 == 0 && a->v_stride[i] % 8 == 0, FM_ERR_INVALID_ARGUMENT, "fm_kv_write: strides are not multiples of 8 elements");
+  p.pay[0] = (uint8_t*)c->k; p.pay[1] = (uint8_t*)c->v; p.scale[0] = c->k_scale; p.scale[1] = c->v_scale;
+  p.src[0] = (const uint16_t*)a->k; p.src[1] = (const uint16_t*)a->v;
+  for (int i = 0; i < 3; ++i) { p.stride[0][i] = a->k_stride[i]; p.stride[1][i] = a->v_stride[i]; }
+  p.width[0] = c->d; p.width[1] = c->dv;
+  p.table = a->page_table; p.start = a->start; p.lengths = a->lengths;
+  p.B = a->B; p.S = a->S;
+  const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
+  const int wmax = c->d > c->dv ? c->d : c->dv;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (bf) return i8 ? launch_write<true, true>(p, c->page_size, wmax, s) : launch_write<true, false>(p, c->page_size, wmax, s);
+  return i8 ? launch_write<false, true>(p, c->page_size, wmax, s) : launch_write<false, false>(p, c->page_size, wmax, s);
+}
+
+extern "C" FM_API int fm_kv_read(const fm_kv_cache* c, const fm_kv_args* a, void* stream) {
+  KvReadParams p;
+  const int rc = kv_geometry(c, a, &p.g);
+  if (rc) return rc;
+  if (a->B == 0 || a->S == 0) return FM_OK;
+  FM_REQUIRE(a->k_out && a->v_out && a->start && a->seqlens, FM_ERR_INVALID_ARGUMENT, "fm_kv_read: an output, start or seqlens is NULL");
+  FM_REQUIRE(((uintptr_t)a->k_out & 15) == 0 && ((uintptr_t)a->v_out & 15) == 0, FM_ERR_INVALID_ARGUMENT, "fm_kv_read: an output is not 16-byte aligned");
+  p.pay[0] = (const uint8_t*)c->k; p.pay[1] = (const uint8_t*)c->v; p.scale[0] = c->k_scale; p.scale[1] = c->v_scale;
+  p.dst[0] = (uint16_t*)a->k_out; p.dst[1] = (uint16_t*)a->v_out;
+  p.width[0] = c->d; p.width[1] = c->dv;
+  p.table = a->page_table; p.start = a->start; p.seqlens = a->seqlens;
+  p.B = a->B; p.S = a->S;
+  const int64_t units = (int64_t)a->S * c->Hkv * ((c->d > c->dv ? c->d : c->dv) / 8), per = 256 * READ_ILP;
+  FM_REQUIRE((units + per - 1) / per <= INT_MAX, FM_ERR_UNSUPPORTED, "fm_kv_read: too many tokens for one call");
+  const dim3 grid((unsigned)((units + per - 1) / per), a->B, 2);
+  const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (bf) { if (i8) kv_read_kernel<true, true><<<grid, 256, 0, s>>>(p); else kv_read_kernel<true, false><<<grid, 256, 0, s>>>(p); }
+  else { if (i8) kv_read_kernel<false, true><<<grid, 256, 0, s>>>(p); else kv_read_kernel<false, false><<<grid, 256, 0, s>>>(p); }
+  count_launches(1);
+  FM_CUDA_TRY(cudaGetLastError());
+  return FM_OK;
+}
+
+extern "C" FM_API int fm_kv_bounds(const fm_kv_cache* c, const fm_kv_args* a, int cols, int32_t* shift, int32_t* bounds, void* stream) {
+  KvBoundsParams p;
+  const int rc = kv_geometry(c, a, &p.g);
+  if (rc) return rc;
+  FM_REQUIRE(cols >= a->S && cols <= INT_MAX - 65536, FM_ERR_INVALID_ARGUMENT, "fm_kv_bounds: %d columns for %d query rows", cols, a->S);
+  FM_REQUIRE(a->window >= 0 && (a->causal || a->window == 0), FM_ERR_INVALID_ARGUMENT, "fm_kv_bounds: window %d (causal %d)", a->window, a->causal);
+  if (a->B == 0 || cols == 0) return FM_OK;
+  FM_REQUIRE(a->seqlens && shift && bounds, FM_ERR_INVALID_ARGUMENT, "fm_kv_bounds: seqlens, shift or bounds is NULL");
+  FM_REQUIRE(((uintptr_t)bounds & 7) == 0, FM_ERR_INVALID_ARGUMENT, "fm_kv_bounds: bounds is not 8-byte aligned");
+  p.seqlens = a->seqlens; p.lengths = a->lengths; p.table = a->page_table;
+  p.shift = shift; p.bounds = bounds;
+  p.B = a->B; p.Sq = a->S; p.cols = cols; p.causal = a->causal; p.window = a->window;
+  kv_bounds_kernel<<<dim3((unsigned)((cols + 255) / 256), a->B), 256, 0, (cudaStream_t)stream>>>(p);
+  count_launches(1);
+  FM_CUDA_TRY(cudaGetLastError());
+  return FM_OK;
+}

@@ -1,0 +1,293 @@
+// Native host of the operators around attention: norm and rotation of q and k with its autograd node, the 8-bit paged
+// cache, attention over it.  Checks, allocations and calls into the C ABI; a decode step makes three such calls in a few
+// microseconds each, which is what its kernels take.
+#include "fm_torch.h"
+
+#include <cmath>
+#include <cstring>
+
+namespace fm_host {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+namespace {
+
+constexpr const char* kNoCpu = "flashmask_b200 runs on CUDA (sm_100a) tensors only; there is no CPU path";
+
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+// t [B, S, H, D] as the kernels read it in 16-byte vectors: rows contiguous, every stride a multiple of 8, base aligned.
+Tensor vec_rows(const Tensor& t) {
+  if (t.numel() == 0) return t;
+  bool ok = t.stride(-1) == 1 && aligned16(t);
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % 8 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// (a dimension of one element may carry any stride)
+void vec_strides(int64_t* out, const Tensor& t) { for (int i = 0; i < 3; ++i) out[i] = t.size(i) == 1 ? 0 : t.stride(i); }
+
+Tensor packed(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return c.numel() == 0 || aligned16(c) ? c : c.clone();
+}
+
+// ---------------------------------------------------------------------------- norm and rotation
+fm_norm_rotary_args norm_args(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
+                              const Tensor& sin, const Tensor& pos, double eps, bool interleaved) {
+  fm_norm_rotary_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.B = (int)q.size(0); a.S = (int)q.size(1); a.Hq = (int)q.size(2); a.Hk = (int)k.size(2); a.d = (int)q.size(3);
+  a.rot = 2 * (int)cos.size(1);
+  a.dtype = dtype_code(q);
+  a.interleaved = interleaved;
+  a.table = (int)cos.size(0);
+  a.eps = (float)eps;
+  a.q = q.data_ptr(); a.k = k.data_ptr();
+  if (qw.defined()) { a.q_weight = qw.data_ptr(); a.weight_f32 = qw.scalar_type() == at::kFloat; }
+  if (kw.defined()) { a.k_weight = kw.data_ptr(); a.weight_f32 = kw.scalar_type() == at::kFloat; }
+  a.cos = cos.data_ptr<float>(); a.sin = sin.data_ptr<float>();
+  if (pos.defined()) {
+    a.positions = pos.data_ptr();
+    a.positions_64 = pos.scalar_type() == at::kLong;
+    a.positions_stride = pos.dim() == 2 && pos.size(0) > 1 ? pos.stride(0) : 0;
+  }
+  vec_strides(a.q_stride, q); vec_strides(a.k_stride, k);
+  return a;
+}
+
+class NormRotary : public torch::autograd::Function<NormRotary> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Variable& q_in, const Variable& k_in, const std::optional<Tensor>& qw_in,
+                               const std::optional<Tensor>& kw_in, const Tensor& cos_in, const Tensor& sin_in,
+                               const std::optional<Tensor>& pos_in, double eps, bool interleaved) {
+    const c10::cuda::CUDAGuard guard(q_in.device());
+    const Tensor q = vec_rows(q_in), k = vec_rows(k_in), cos = packed(cos_in), sin = packed(sin_in);
+    const Tensor qw = qw_in ? packed(*qw_in) : Tensor(), kw = kw_in ? packed(*kw_in) : Tensor();
+    const Tensor pos = pos_in ? (pos_in->stride(-1) == 1 ? *pos_in : pos_in->contiguous()) : Tensor();
+    Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+    fm_norm_rotary_args a = norm_args(q, k, qw, kw, cos, sin, pos, eps, interleaved);
+    a.q_out = qo.data_ptr(); a.k_out = ko.data_ptr();
+    vec_strides(a.qo_stride, qo); vec_strides(a.ko_stride, ko);
+    check(fm_norm_rotary_fwd(&a, stream_of(q)), "fm_norm_rotary_fwd");
+    ctx->save_for_backward({q, k, qw, kw, cos, sin, pos});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["dqw"] = qw_in && qw_in->requires_grad();
+    ctx->saved_data["dkw"] = kw_in && kw_in->requires_grad();
+    return {qo, ko};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &qw = s[2], &kw = s[3];
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Tensor gq = vec_rows(grads[0]), gk = vec_rows(grads[1]);
+    fm_norm_rotary_args a = norm_args(q, k, qw, kw, s[4], s[5], s[6], ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dqw, dkw, ws;
+    a.q_out = dq.data_ptr(); a.k_out = dk.data_ptr();
+    a.d_q = gq.data_ptr(); a.d_k = gk.data_ptr();
+    vec_strides(a.qo_stride, dq); vec_strides(a.ko_stride, dk); vec_strides(a.dq_stride, gq); vec_strides(a.dk_stride, gk);
+    if (qw.defined() && ctx->saved_data["dqw"].toBool()) { dqw = at::empty(qw.sizes(), qw.options()); a.dq_weight = dqw.data_ptr(); }
+    if (kw.defined() && ctx->saved_data["dkw"].toBool()) { dkw = at::empty(kw.sizes(), kw.options()); a.dk_weight = dkw.data_ptr(); }
+    if (dqw.defined() || dkw.defined()) {
+      a.workspace_bytes = fm_norm_rotary_bwd_workspace_bytes(&a);
+      ws = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
+      a.workspace = ws.data_ptr();
+    }
+    check(fm_norm_rotary_bwd(&a, stream_of(q)), "fm_norm_rotary_bwd");
+    return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const std::optional<Tensor>& qw, const std::optional<Tensor>& kw,
+                                      const Tensor& cos, const Tensor& sin, const std::optional<Tensor>& pos, double eps,
+                                      bool interleaved) {
+  TORCH_CHECK(q.is_cuda(), kNoCpu);
+  require(q.dim() == 4 && k.dim() == 4, "query and key must be [B, S, H, D]");
+  require(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3), "key's shape does not match query");
+  require(q.scalar_type() == k.scalar_type(), "query and key must share a dtype");
+  require(q.device() == k.device() && q.device() == cos.device() && q.device() == sin.device(), "all tensors must be on the device of query");
+  dtype_code(q);
+  const int64_t d = q.size(3);
+  require(cos.dim() == 2 && cos.sizes() == sin.sizes() && 2 * cos.size(1) <= d, "cos and sin must be [positions, n] with 2 n <= head dim");
+  require(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "cos and sin must be float32");
+  require(!cos.requires_grad() && !sin.requires_grad(), "cos and sin take no gradient");
+  for (const auto* w : {&qw, &kw}) {
+    if (!*w) continue;
+    require((*w)->dim() == 1 && (*w)->size(0) == d, "weights must be [head dim]");
+    require((*w)->device() == q.device(), "weights must be on the device of query");
+    require((*w)->scalar_type() == at::kFloat || (*w)->scalar_type() == q.scalar_type(), "weights must be float32 or of query's dtype");
+  }
+  require(!qw || !kw || (*qw).scalar_type() == (*kw).scalar_type(), "weights must share a dtype");
+  if (pos) {
+    require(pos->device() == q.device(), "positions must be on the device of query");
+    require(pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong, "positions must be int32 or int64");
+    require((pos->dim() == 1 && pos->size(0) == q.size(1)) ||
+            (pos->dim() == 2 && pos->size(1) == q.size(1) && (pos->size(0) == q.size(0) || pos->size(0) == 1)), "positions must be [B, S] or [S]");
+  }
+  pybind11::gil_scoped_release nogil;
+  const variable_list r = NormRotary::apply(q, k, qw, kw, cos, sin, pos, eps, interleaved);
+  return {r[0], r[1]};
+}
+
+// ---------------------------------------------------------------------------- cache
+struct Cache { const Tensor &k, &v, &ks, &vs; };
+
+fm_kv_cache cache_of(const Cache& c) {
+  fm_kv_cache r;
+  require(c.k.dim() == 4 && c.v.dim() == 4 && c.k.sizes().slice(0, 3) == c.v.sizes().slice(0, 3),
+          "cache k and v must be [num_pages, Hkv, page_size, D]");
+  require(c.k.scalar_type() == c.v.scalar_type() && (c.k.scalar_type() == at::kFloat8_e4m3fn || c.k.scalar_type() == at::kChar),
+          "cache k and v must be float8_e4m3fn or int8");
+  require(c.ks.scalar_type() == at::kFloat && c.vs.scalar_type() == at::kFloat && c.ks.sizes() == c.k.sizes().slice(0, 2) &&
+          c.vs.sizes() == c.k.sizes().slice(0, 2), "cache scales must be float32 [num_pages, Hkv]");
+  require(c.k.is_contiguous() && c.v.is_contiguous() && c.ks.is_contiguous() && c.vs.is_contiguous(), "cache tensors must be contiguous");
+  require(c.k.device() == c.v.device() && c.k.device() == c.ks.device() && c.k.device() == c.vs.device(), "cache tensors must be on one device");
+  TORCH_CHECK_NOT_IMPLEMENTED(c.k.size(0) <= INT_MAX && c.k.size(1) <= INT_MAX, "cache too large");
+  r.k = c.k.data_ptr(); r.v = c.v.data_ptr(); r.k_scale = c.ks.data_ptr<float>(); r.v_scale = c.vs.data_ptr<float>();
+  r.num_pages = (int)c.k.size(0); r.Hkv = (int)c.k.size(1); r.page_size = (int)c.k.size(2); r.d = (int)c.k.size(3); r.dv = (int)c.v.size(3);
+  r.dtype = c.k.scalar_type() == at::kChar ? FM_CACHE_INT8 : FM_CACHE_E4M3;
+  return r;
+}
+
+const int32_t* ints(const std::optional<Tensor>& t, int64_t B, const Tensor& like, const char* msg, Tensor* keep) {
+  if (!t) return nullptr;
+  require(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->device() == like.device(), msg);
+  *keep = t->contiguous();
+  return keep->data_ptr<int>();
+}
+
+fm_kv_args kv_args(const Cache& c, const Tensor& table, int64_t B, int64_t S, Tensor* keep) {
+  fm_kv_args a;
+  std::memset(&a, 0, sizeof(a));
+  require(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == B && table.device() == c.k.device(),
+          "page_table must be int32 [B, pages] on the cache's device");
+  TORCH_CHECK_NOT_IMPLEMENTED(B <= 65535 && S <= INT_MAX - 65536 && table.size(1) <= INT_MAX, "too many sequences, rows or pages");
+  *keep = table.stride(1) == 1 || table.size(1) <= 1 ? table : table.contiguous();
+  if (table.size(0) > 1 && keep->stride(0) < table.size(1)) *keep = keep->contiguous();
+  a.B = (int)B; a.S = (int)S;
+  a.max_pages = (int)table.size(1);
+  a.table_stride = keep->stride(0);
+  a.page_table = keep->data_ptr<int>();
+  return a;
+}
+
+void no_gradient(const Tensor& t, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no gradient: call it under torch.no_grad()");
+}
+
+void kv_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs, const Tensor& key_in, const Tensor& value_in,
+              const Tensor& table, const Tensor& start, const std::optional<Tensor>& lengths) {
+  const Cache c{ck, cv, cks, cvs};
+  TORCH_CHECK(ck.is_cuda() && key_in.is_cuda(), kNoCpu);
+  const fm_kv_cache f = cache_of(c);
+  require(key_in.dim() == 4 && value_in.dim() == 4 && key_in.sizes().slice(0, 3) == value_in.sizes().slice(0, 3) && key_in.size(2) == f.Hkv &&
+          key_in.size(3) == f.d && value_in.size(3) == f.dv, "key and value must be [B, S, Hkv, D] of the cache's heads");
+  require(key_in.scalar_type() == value_in.scalar_type(), "key and value must share a dtype");
+  require(key_in.device() == ck.device() && value_in.device() == ck.device(), "key and value must be on the cache's device");
+  no_gradient(key_in, "kv_cache_write");
+  no_gradient(value_in, "kv_cache_write");
+  const c10::cuda::CUDAGuard guard(ck.device());
+  Tensor keep[3];
+  fm_kv_args a = kv_args(c, table, key_in.size(0), key_in.size(1), &keep[0]);
+  a.dtype = dtype_code(key_in);
+  a.start = ints(start, a.B, ck, "start must be int32 [B] on the cache's device", &keep[1]);
+  a.lengths = ints(lengths, a.B, ck, "lengths must be int32 [B] on the cache's device", &keep[2]);
+  const Tensor key = vec_rows(key_in), value = vec_rows(value_in);
+  a.k = key.data_ptr(); a.v = value.data_ptr();
+  vec_strides(a.k_stride, key); vec_strides(a.v_stride, value);
+  check(fm_kv_write(&f, &a, stream_of(ck)), "fm_kv_write");
+}
+
+std::pair<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs, const Tensor& table,
+                                  const Tensor& start, const Tensor& seqlens, int64_t length, at::ScalarType dtype) {
+  const Cache c{ck, cv, cks, cvs};
+  TORCH_CHECK(ck.is_cuda(), kNoCpu);
+  const fm_kv_cache f = cache_of(c);
+  require(length >= 0, "length must not be negative");
+  const c10::cuda::CUDAGuard guard(ck.device());
+  Tensor keep[3];
+  fm_kv_args a = kv_args(c, table, table.size(0), length, &keep[0]);
+  a.start = ints(start, a.B, ck, "start must be int32 [B] on the cache's device", &keep[1]);
+  a.seqlens = ints(seqlens, a.B, ck, "seqlens must be int32 [B] on the cache's device", &keep[2]);
+  const auto opt = ck.options().dtype(dtype);
+  Tensor k = at::empty({a.B, length, f.Hkv, f.d}, opt), v = at::empty({a.B, length, f.Hkv, f.dv}, opt);
+  a.dtype = dtype_code(k);
+  a.k_out = k.data_ptr(); a.v_out = v.data_ptr();
+  check(fm_kv_read(&f, &a, stream_of(ck)), "fm_kv_read");
+  return {k, v};
+}
+
+// Rows (queries x heads of a group) up to which the cache is read by the kernel for few rows.  Beyond, the tokens are
+// read back once into dense 16-bit tensors and the dense forward, which feeds the tensor cores, takes the call.
+constexpr int64_t kFewRows = 64;
+
+std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs,
+                                       const Tensor& table, const Tensor& seqlens, const std::optional<Tensor>& lengths,
+                                       const std::optional<Tensor>& sink, bool causal, int64_t window, std::optional<double> scale_in,
+                                       int64_t max_seqlen) {
+  const Cache c{ck, cv, cks, cvs};
+  TORCH_CHECK(ck.is_cuda() && query.is_cuda(), kNoCpu);
+  const fm_kv_cache f = cache_of(c);
+  require(query.dim() == 4 && query.size(3) == f.d, "query must be [B, S, H, D] of the cache's head dim");
+  require(f.Hkv > 0 && query.size(2) % f.Hkv == 0 && query.size(2) > 0, "num q heads must be a multiple of num kv heads");
+  require(query.device() == ck.device(), "query must be on the cache's device");
+  if (sink) require(sink->numel() == query.size(2), "sink must have one logit per q head");
+  TORCH_CHECK_VALUE(window >= 0 && (causal || window == 0), "window_size needs causal=True and at least one token");
+  no_gradient(query, "kv_cache_attention");
+  const c10::cuda::CUDAGuard guard(ck.device());
+  Tensor keep[3];
+  const int64_t B = query.size(0), S = query.size(1), Hq = query.size(2);
+  fm_kv_args a = kv_args(c, table, B, S, &keep[0]);
+  a.Hq = (int)Hq;
+  a.dtype = dtype_code(query);
+  a.seqlens = ints(seqlens, B, ck, "seqlens must be int32 [B] on the cache's device", &keep[1]);
+  a.lengths = ints(lengths, B, ck, "q_lengths must be int32 [B] on the cache's device", &keep[2]);
+  a.causal = causal;
+  a.window = (int)std::min<int64_t>(window, INT_MAX);
+  const double scale = scale_in ? *scale_in : 1.0 / std::sqrt((double)f.d);
+  a.softmax_scale = (float)scale;
+  void* stream = stream_of(ck);
+  const Tensor sink32 = sink ? sink_fp32(*sink, query) : Tensor();
+  if (S * (Hq / f.Hkv) > kFewRows && B > 0) {
+    int64_t cols = std::min<int64_t>(max_seqlen, (int64_t)a.max_pages * f.page_size);
+    // (with rows that do not count the real ones stand up to S columns further left)
+    cols = std::max<int64_t>(lengths ? cols + S : cols, S);
+    const auto i32 = table.options();
+    const Tensor shift = at::empty({B}, i32), bounds = at::empty({B, 1, cols, causal ? 1 : 2}, i32);
+    check(fm_kv_bounds(&f, &a, (int)cols, shift.data_ptr<int>(), bounds.data_ptr<int>(), stream), "fm_kv_bounds");
+    const Tensor k = at::empty({B, cols, f.Hkv, f.d}, query.options()), v = at::empty({B, cols, f.Hkv, f.dv}, query.options());
+    fm_kv_args r = a;
+    r.S = (int)cols; r.start = shift.data_ptr<int>(); r.k_out = k.data_ptr(); r.v_out = v.data_ptr();
+    check(fm_kv_read(&f, &r, stream), "fm_kv_read");
+    return attention(query.detach(), k, v, bounds, sink32.defined() ? std::optional<Tensor>(sink32) : std::nullopt, scale, causal, 0);
+  }
+  const Tensor q = vec_rows(query);
+  const Tensor out = at::empty({B, S, Hq, f.dv}, q.options()), lse = at::empty({B, Hq, S}, q.options().dtype(at::kFloat));
+  a.workspace_bytes = fm_kv_attention_workspace_bytes(&f, &a);
+  const Tensor ws = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.q = q.data_ptr(); a.o = out.data_ptr(); a.lse = lse.data_ptr<float>();
+  vec_strides(a.q_stride, q);
+  if (sink32.defined()) a.sink = sink32.data_ptr<float>();
+  check(fm_kv_attention(&f, &a, stream), "fm_kv_attention");
+  return {out, lse};
+}
+
+}  // namespace
+
+void register_cache(pybind11::module_& m) {
+  m.def("norm_rotary", &norm_rotary);
+  m.def("kv_write", &kv_write);
+  m.def("kv_read", [](const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table, const Tensor& start,
+                      const Tensor& seqlens, int64_t length, bool fp16) {
+    return kv_read(k, v, ks, vs, table, start, seqlens, length, fp16 ? at::kHalf : at::kBFloat16);
+  });
+  m.def("kv_attention", &kv_attention);
+}
+
+}  // namespace fm_host

@@ -407,6 +407,110 @@ FM_API int fm_cp_reduce_partials(const void* const* parts, int n_parts, void* ou
  */
 FM_API int fm_bwd_static_scratch(const fm_attn_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Before attention: norm of every head of q and k, rotation by position
+ * ------------------------------------------------------------------------ */
+
+/* For every row x of d values (a head of a token): u = x / sqrt(mean(x^2) + eps) * weight, then the pairs (a, b) of the
+ * first `rot` values turn by the angles of the token's position: (a cos - b sin, b cos + a sin).  A pair is
+ * (i, i + rot / 2), or (2 i, 2 i + 1) with `interleaved`.  q and k go through one launch.  Sums and products are fp32;
+ * results are rounded once.  A position outside of the tables makes its rows NaN.
+ * Strides are in elements (batch, token, head), multiples of 8; tensors, weights and tables are 16-byte aligned; the
+ * head dim is contiguous, a multiple of 16 up to 512, `rot` a multiple of 16.  No counterpart in the reference, which
+ * begins at attention. */
+typedef struct fm_norm_rotary_args {
+  int32_t B, S, Hq, Hk, d, rot;
+  int32_t dtype;            /* FM_DTYPE_* of q, k, outputs and gradients          */
+  int32_t interleaved;
+  int32_t weight_f32;       /* weights and their gradients: 1 = fp32, 0 = dtype   */
+  int32_t table;            /* positions in cos and sin                           */
+  int32_t positions_64;     /* positions are int64 (else int32)                   */
+  float eps;
+  const void* q; const void* k;
+  const void* q_weight; const void* k_weight;    /* [d], or NULL: ones            */
+  const float* cos; const float* sin;            /* [table, rot / 2]              */
+  const void* positions;    /* [B, S], or NULL: token i stands at position i      */
+  int64_t positions_stride; /* elements from one sequence to the next (0: shared) */
+  void* q_out; void* k_out;                      /* backward: dL/dq, dL/dk        */
+  const void* d_q; const void* d_k;              /* backward: dL/dq_out, dL/dk_out */
+  void* dq_weight; void* dk_weight;              /* backward: [d], or NULL        */
+  void* workspace; size_t workspace_bytes;       /* backward with a weight's gradient */
+  int64_t q_stride[3], k_stride[3], qo_stride[3], ko_stride[3], dq_stride[3], dk_stride[3];
+} fm_norm_rotary_args;
+
+FM_API int fm_norm_rotary_fwd(const fm_norm_rotary_args* args, void* stream);
+/* The backward takes the forward's inputs and the gradients of its outputs; bitwise reproducible.  The workspace
+ * holds partial sums of the weights' gradients and needs no initialisation; without those gradients it may be NULL. */
+FM_API size_t fm_norm_rotary_bwd_workspace_bytes(const fm_norm_rotary_args* args);
+FM_API int fm_norm_rotary_bwd(const fm_norm_rotary_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Generation: a paged cache of keys and values in 8 bits, and attention over it
+ * ------------------------------------------------------------------------ */
+
+#define FM_CACHE_E4M3 0
+#define FM_CACHE_INT8 1
+
+/* k [num_pages, Hkv, page_size, d], v [num_pages, Hkv, page_size, dv], one byte a value; k_scale, v_scale
+ * [num_pages, Hkv] fp32; all contiguous.  A stored value is payload * scale, and a scale is a power of two: the least
+ * 2^e with max |x| <= 448 * 2^e (e4m3; -64 <= e <= 119) or 127 * 2^e (int8; e <= 121) over the tokens of the page.
+ * page_size is 16, 32, 64 or 128; d and dv are multiples of 16 up to 128, or 192 / 128, or 256 / 256. */
+typedef struct fm_kv_cache {
+  void* k; void* v; float* k_scale; float* v_scale;
+  int32_t num_pages, page_size, Hkv, d, dv, dtype;    /* dtype: FM_CACHE_* */
+} fm_kv_cache;
+
+/* Position p of sequence b is slot p % page_size of page page_table[b][p / page_size].  A position behind the page
+ * table, or whose page is not in [0, num_pages), is no token: it is not written, reads as zeros, and attention does not
+ * see it.  seqlens beyond the page table count as its length, negative ones as 0. */
+typedef struct fm_kv_args {
+  int32_t B, S;             /* sequences, and rows of each in q / k / v / the outputs */
+  int32_t Hq, dtype;        /* FM_DTYPE_* of the 16-bit tensors                    */
+  int32_t max_pages;        /* columns of page_table                              */
+  int32_t causal, window;   /* attention: see fm_kv_attention                      */
+  float softmax_scale;
+  int64_t table_stride;     /* elements between the rows of page_table             */
+  const int32_t* page_table;
+  const int32_t* seqlens;   /* [B] tokens of every sequence, new ones included (read, attention) */
+  const int32_t* start;     /* [B] position of row 0 (write, read)                 */
+  const int32_t* lengths;   /* [B] rows of S that count, or NULL: all (write, attention) */
+  const void* q; const void* k; const void* v;
+  void* o; float* lse; void* k_out; void* v_out;
+  const float* sink;
+  void* workspace; size_t workspace_bytes;
+  int64_t q_stride[3], k_stride[3], v_stride[3];      /* elements: batch, row, head */
+} fm_kv_args;
+
+/* Offset of a position in the payload (elements from k, or from v with `value`), or -1 where the position is no token:
+ * what the kernels compute before they touch a page.  HOST pointers in args->page_table. */
+FM_API int64_t fm_kv_locate(const fm_kv_cache* cache, const fm_kv_args* args, int b, int head, int64_t pos, int value);
+
+/* Writes rows i < lengths[b] of k [B, S, Hkv, d] and v [B, S, Hkv, dv] at positions start[b] + i, rounded to nearest
+ * even on the page's grid.  A page whose slot 0 is written begins anew; in the others the scale keeps its size or
+ * grows with the new tokens, and what was there before is then rounded on the new grid.  NaN and infinities read back
+ * as NaN: the value itself in e4m3, the whole page of that head in int8, whose scale becomes NaN until the page begins
+ * anew.  A page must not be written for two sequences in one call. */
+FM_API int fm_kv_write(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
+
+/* k_out [B, S, Hkv, d], v_out [B, S, Hkv, dv] (contiguous): the tokens at positions start[b] + i, zeros where the
+ * position is below 0, at seqlens[b] or beyond, or no token.  Exact in bf16; fp16 saturates at 65504. */
+FM_API int fm_kv_read(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
+
+/* o [B, S, Hq, dv] (contiguous) and lse [B, Hq, S] of q [B, S, Hq, d] against the cache.  Rows i < n = lengths[b] stand
+ * at positions seqlens[b] - n + i and see the positions up to their own (causal) and, with window > 0, the last
+ * `window` of those; without `causal` they see all.  A row that sees nothing gives 0 and lse -inf (with a sink: the
+ * sink).  sink [Hq] fp32 or NULL joins every denominator.
+ * The keys are dealt evenly to the CTAs whatever the lengths, and partial results are merged by a second kernel;
+ * the host never needs the lengths.  The workspace needs no initialisation and serves one call at a time. */
+FM_API size_t fm_kv_attention_workspace_bytes(const fm_kv_cache* cache, const fm_kv_args* args);
+FM_API int fm_kv_attention(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
+
+/* For attention with many query rows over tokens read back into dense tensors of `cols` >= S columns: the position of
+ * column 0 of every sequence (`shift` [B], the start of an fm_kv_read of `cols` rows) and the column bounds
+ * [B, 1, cols, 1 (causal) | 2] with which fm_fwd gives what fm_kv_attention gives. */
+FM_API int fm_kv_bounds(const fm_kv_cache* cache, const fm_kv_args* args, int cols, int32_t* shift, int32_t* bounds,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
