@@ -9,13 +9,13 @@
 //   V: lane (g, t) loads chunk g of keys 2t, 2t + 1, 2t + 8, 2t + 9; byte pairs of two keys are the A operand's pairs
 //      along the keys, and byte 2j, 2j + 1 of chunk g are rows g, g + 8 of O^T's tile j.
 //   P^T: the S^T fragment, rounded to fp16 and transposed in registers (movmatrix).
-// q in bf16 is brought to fp16 by a power of two per row; p is in (0, 2^8], where fp16 has three bits more than bf16.
+// q in bf16 is brought to fp16 by a power of two per row; p is in (0, 2^15], where fp16 has three bits more than bf16.
 //
 // Scales.  A page's k scale multiplies the scores.  Its v scale joins the exponent: with x = s + log2(vs) the kernel
 // keeps m = max x and p' = 2^(x - m), so that p' V8 sums are in units of 2^m for every page, and the denominator takes
 // p' / vs.  Powers of two: both are exact.
 //
-// Work.  The units (8 warps x 16 keys) of all items are laid out end to end and dealt evenly to one wave of CTAs, each
+// Work.  The units (4 warps x 32 keys) of all items are laid out end to end and dealt evenly to one wave of CTAs, each
 // a contiguous range: sequences of any lengths load the chip evenly, and nothing about the lengths is needed on the
 // host.  A CTA leaves a partial result (fp32 O, l, m) where its range cuts an item; kv_attn_merge_kernel joins them.
 // Bound by HBM: (d + dv) bytes a key.
@@ -34,12 +34,48 @@ struct KvAttnParams {
   int B, S, Hq, G, d, dv, causal, window, bf16;
   int row_tiles;                 // of ROWS rows, per kv head
   float scale_log2;
-  int* pre;                      // workspace: [B + 1] first unit of every sequence
   float* part_o; float* part_ml; // workspace: [2 n_cta][ROWS][DV], [2 n_cta][ROWS][2]
   int n_cta;
 };
 
-constexpr int KV_WARPS = 8, KV_UNIT = 16 * KV_WARPS;
+// A warp works on blocks of 32 keys (two groups of 16), the four blocks of a unit side by side.
+constexpr int KV_WARPS = 4, KV_BLOCK = 32, KV_UNIT = KV_BLOCK * KV_WARPS, KV_INFO = 64;
+
+// DK = ceil(d / 64), VC = bytes of a lane's chunk of V (dv <= 8 VC), NT = column tiles of 8 rows.
+// Several CTAs share an SM: while one waits or joins its warps the others' copies and products go on.
+template <int DK, int VC, int NT>
+struct KvCfg {
+  static constexpr int KP = DK * 64, VP = VC * 8;                // bytes of a key's and a value's row in shared memory
+  static constexpr int GROUP = 16 * (KP + VP), STAGE = 2 * GROUP;          // a group and a block of a warp
+  static constexpr int CTAS = VC > 16 ? 1 : (DK > 2 ? 2 : (DK == 1 ? (NT == 1 ? 4 : (NT == 2 ? 3 : 2)) : (NT == 1 ? 3 : 2)));    // by their registers
+  static constexpr int STAGES = (CTAS == 1 ? 192 : (CTAS == 2 ? (NT > 2 ? 80 : 96) : (CTAS == 3 ? 64 : 48))) * 1024 / (KV_WARPS * STAGE);
+  static constexpr int RING = KV_WARPS * STAGES * STAGE;
+  static constexpr int ROWS = 8 * NT, DV = 8 * VC, MT = VC / 2;  // MT row tiles of O^T
+  static constexpr int JOIN = STAGE / (MT * 512) < NT ? STAGE / (MT * 512) : NT;    // column tiles whose O fits a stage
+  static constexpr int Q = NT * DK * 4 * 32 * 8;                 // Q^T fragments
+  static constexpr int FIXED = RING + Q + KV_WARPS * KV_INFO * 16 + 2 * KV_WARPS * ROWS * 4 + ROWS * 12;   // .., info, m, l, limits and scales
+  static_assert(STAGES >= 2 && 2 * STAGES <= KV_INFO - 32, "a block is copied while another is used");
+  static_assert(JOIN > 0 && NT % JOIN == 0 && NT <= KV_WARPS, "O fits the stage of the last block; a warp for every tile of queries");
+};
+
+// Byte offsets of 16-byte chunk c of row r of a group in shared memory.  The reads of eight lanes that are served
+// together go to chunks t .. t + 3 of two neighbouring keys, and to chunks g, g + 1 of values 2t, t = 0 .. 3: the
+// permutations put these on different banks.
+template <int DK>
+__device__ __forceinline__ uint32_t k_at(int r, int c) { return r * (DK * 64) + ((DK & 1 ? c : c ^ ((r & 1) << 2)) << 4); }
+template <int VC>
+__device__ __forceinline__ uint32_t v_at(int r, int c) { return r * (VC * 8) + ((VC == 8 ? c ^ (r >> 1 & 3) : c ^ ((r >> 1 & 3) << 1)) << 4); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
 
 // What the rows of a sequence may see: rows i < n stand at p0 + i; keys [lo, hi) are seen by one of them at least.
 struct KvRange { int len, n, p0, lo, hi; };
@@ -49,7 +85,7 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnParams& p, int b) {
   r.n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   r.p0 = r.len - r.n;
   r.hi = r.n > 0 ? r.len : 0;
-  r.lo = p.window > 0 ? min(max((int64_t)r.p0 - p.window + 1, (int64_t)0), (int64_t)r.hi) & ~15 : 0;
+  r.lo = p.window > 0 ? min(max((int64_t)r.p0 - p.window + 1, (int64_t)0), (int64_t)r.hi) & ~(KV_BLOCK - 1) : 0;
   return r;
 }
 __device__ __forceinline__ int kv_units(const KvRange& r) { return max(1, (r.hi - r.lo + KV_UNIT - 1) / KV_UNIT); }
@@ -71,30 +107,35 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 // 0x80 in every byte of w that is an e4m3 NaN (0x7f, 0xff).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
+// What a range of units of one item is: the item, and which of its keys.
+struct KvSegment { int b, h, row0, units, u0, u1, key0; KvRange r; };
 
-// DK = ceil(d / 64), VC = bytes of a lane's chunk of V (dv <= 8 VC), NT = column tiles of 8 rows.
-template <int DK, int VC, int NT, bool INT8>
-__global__ void __launch_bounds__(KV_WARPS * 32, 1) kv_attn_kernel(const KvAttnParams p) {
-  constexpr int MT = VC / 2, ROWS = 8 * NT, DV = 8 * VC, VW = VC / 4;       // row tiles of O^T, words of V per lane and key
-  extern __shared__ __align__(16) float smem[];
-  float* s_o = smem;                                  // [warps][MT * 4][32]
-  float* s_m = s_o + KV_WARPS * MT * 128;             // [warps][ROWS]
+// FULL: d = 64 DK and dv = 8 VC, known to the compiler.
+// The loops over chunks of the head dim and over the two groups stay loops: short calls run every instruction once or
+// twice, and wait for instructions more than for anything else.
+template <int DK, int VC, int NT, bool INT8, bool FULL>
+__global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_attn_kernel(const __grid_constant__ KvAttnParams p) {
+  using Cfg = KvCfg<DK, VC, NT>;
+  constexpr int MT = Cfg::MT, ROWS = Cfg::ROWS, DV = Cfg::DV, VW = VC / 4, STAGES = Cfg::STAGES, JOIN = Cfg::JOIN;    // VW words of V per lane and key
+  extern __shared__ __align__(128) unsigned char smem[];
+  uint2* s_q = reinterpret_cast<uint2*>(smem + Cfg::RING);                  // [NT][DK][4][32]
+  float4* s_info = reinterpret_cast<float4*>(smem + Cfg::RING + Cfg::Q);    // [warps][KV_INFO]
+  float* s_m = reinterpret_cast<float*>(s_info + KV_WARPS * KV_INFO);       // [warps][ROWS]
   float* s_l = s_m + KV_WARPS * ROWS;                 // [warps][ROWS]
-  int* s_pre = reinterpret_cast<int*>(s_l + KV_WARPS * ROWS);               // [B + 1]
+  int2* s_lim = reinterpret_cast<int2*>(s_l + KV_WARPS * ROWS);             // [ROWS] keys that a row sees
+  float* s_f = reinterpret_cast<float*>(s_lim + ROWS);                      // [ROWS] scale of a row of q
+  int* s_pre = reinterpret_cast<int*>(s_f + ROWS);    // [B + 1] first unit of every sequence
   __shared__ int s_scan[KV_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int d = FULL ? DK * 64 : p.d, dv = FULL ? VC * 8 : p.dv;
+  grid_dep_trigger();                                 // (the merge waits for this kernel's end before it reads anything)
   const int items = p.g.Hkv * p.row_tiles;            // of one sequence
-
-  // first unit of every sequence
+  // sequences b0 .. of this thread; most calls have one at most
+  const int per = (p.B + KV_WARPS * 32 - 1) / (KV_WARPS * 32), b0 = tid * per, b1 = min(b0 + per, p.B);
   {
-    const int per = (p.B + KV_WARPS * 32 - 1) / (KV_WARPS * 32), b0 = tid * per, b1 = min(b0 + per, p.B);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += kv_units(kv_range(p, b)) * items;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) { s_pre[b] = mine; mine += kv_units(kv_range(p, b)) * items; }
     int x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
@@ -102,253 +143,401 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) kv_attn_kernel(const KvAttnP
     __syncthreads();
     int at = x - mine;
     for (int w = 0; w < warp; ++w) at += s_scan[w];
-    for (int b = b0; b < b1; ++b) { s_pre[b] = at; at += kv_units(kv_range(p, b)) * items; }
-    if (b1 == p.B && b0 < b1) s_pre[p.B] = at;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) s_pre[b] += at;
+    if (b1 == p.B && b0 < b1) s_pre[p.B] = at + mine;
     __syncthreads();
   }
-  const int total = s_pre[p.B];
-  if (blockIdx.x == 0)
-    for (int b = tid; b <= p.B; b += KV_WARPS * 32) p.pre[b] = s_pre[b];
-  const int u_end = (int)((int64_t)total * (blockIdx.x + 1) / p.n_cta);
-  int u_at = (int)((int64_t)total * blockIdx.x / p.n_cta);
+  const int total = s_pre[p.B], n_cta = min(p.n_cta, total);            // (never a CTA without a unit between two with one)
+  if (blockIdx.x >= n_cta) return;
+  const int u_begin = (int)((int64_t)total * blockIdx.x / n_cta), n_units = (int)((int64_t)total * (blockIdx.x + 1) / n_cta) - u_begin;
 
-  while (u_at < u_end) {
-    // the item of unit u_at
-    int b = 0;
-    {
-      int hi = p.B;                                   // s_pre[b] <= u_at < s_pre[hi]
-      while (hi - b > 1) { const int mid = (b + hi) >> 1; if (s_pre[mid] <= u_at) b = mid; else hi = mid; }
+  // The part of the item of unit u that this CTA has from u on.
+  auto segment = [&](int u) {
+    KvSegment s;
+    int b = 0, hi = p.B;                              // s_pre[b] <= u < s_pre[hi]
+#pragma unroll 1
+    while (hi - b > 1) { const int mid = (b + hi) >> 1; if (s_pre[mid] <= u) b = mid; else hi = mid; }
+    s.b = b;
+    s.r = kv_range(p, b);
+    s.units = kv_units(s.r);
+    const int in_seq = u - s_pre[b], item = in_seq / s.units;
+    s.u0 = in_seq - item * s.units;
+    s.u1 = min(s.units, s.u0 + u_begin + n_units - u);
+    s.h = item / p.row_tiles;
+    s.row0 = (item - s.h * p.row_tiles) * ROWS;
+    s.key0 = s.r.lo + s.u0 * KV_UNIT;
+    return s;
+  };
+
+  // Groups j = 2 i + (0, 1) of the warp's block in unit u_begin + i.  They are looked up 32 at a time, a lane each and across
+  // items, and kept in shared memory: the index of the group in the cache (-1: none), which the copies need, and (ks,
+  // log2 vs, 1 / vs) behind the first copies.  A group that is none has scores of -inf and values of 0.
+  float4* info = s_info + warp * KV_INFO;
+  int page = -1, head = 0;
+  auto look_up_place = [&](int first) {
+    const int i = (first + lane) >> 1;
+    int at = -1;
+    page = -1;
+    if (i < n_units) {
+      const KvSegment s = segment(u_begin + i);
+      const int key = s.key0 + KV_BLOCK * warp + (lane & 1) * 16;
+      head = s.h;
+      if (key < s.r.hi) page = kv_page(p.g, p.table + s.b * p.g.table_stride, key);
+      if (page >= 0) at = ((page * p.g.Hkv + head) << (p.g.page_log2 - 4)) + ((key & ((1 << p.g.page_log2) - 1)) >> 4);
     }
-    const KvRange r = kv_range(p, b);
-    const int units = kv_units(r), in_seq = u_at - s_pre[b], item = in_seq / units, u0 = in_seq - item * units;
-    const int u1 = min(units, u0 + u_end - u_at), h = item / p.row_tiles, row0 = (item - h * p.row_tiles) * ROWS;
-    const int key0 = r.lo + u0 * KV_UNIT, key1 = min(r.hi, r.lo + u1 * KV_UNIT);
-    const int32_t* trow = p.table + b * p.g.table_stride;
-
-    // Q^T fragments (row g of every tile) and what the lane's columns 2t, 2t + 1 see
-    uint32_t qf[NT][DK][4][2];
-    float f[NT][2], m[NT][2], l[NT][2];
-    int lo[NT][2], hi[NT][2], lo_max = 0, hi_min = INT_MAX;
+    info[(first + lane) & (KV_INFO - 1)].w = __int_as_float(at);
+    __syncwarp();
+  };
+  auto look_up_scale = [&](int first) {
+    float ks = 0.f, vs = 1.f;
+    if (page >= 0) {
+      const int64_t ph = (int64_t)page * p.g.Hkv + head;
+      ks = __ldg(p.ks + ph);
+      vs = __ldg(p.vs + ph);
+    }
+    float4* to = &info[(first + lane) & (KV_INFO - 1)];
+    to->x = ks;
+    to->y = page >= 0 ? log2f(vs) : -INFINITY;
+    to->z = vs > 0.f ? 1.f / vs : 1.f;                     // (not needed of a NaN scale: the scores of the keys that are seen are NaN)
+    __syncwarp();
+  };
+  const uint32_t ring = smem_u32(smem) + warp * STAGES * Cfg::STAGE;
+  // The copies of the warp's block in unit i, 16 bytes a lane; zeros behind the head dim.  One commit for every call.
+  auto fetch = [&](int i, int stage) {
+    if (i < n_units) {
+      if ((i & 15) == 0) look_up_place(2 * i);
+#pragma unroll 1
+      for (int hh = 0; hh < 2; ++hh) {
+        const int at = __float_as_int(info[(2 * i + hh) & (KV_INFO - 1)].w);
+        const uint32_t to = ring + stage * Cfg::STAGE + hh * Cfg::GROUP;
+        const uint8_t *kp = p.k + (int64_t)max(at, 0) * 16 * d, *vp = p.v + (int64_t)max(at, 0) * 16 * dv;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = row0 + nt * 8 + g, i = row / p.G;
-      const bool on = i < p.S;
-      const uint16_t* src = p.q + b * p.qs[0] + i * p.qs[1] + ((int64_t)h * p.G + row - i * p.G) * p.qs[2];
-      uint4 x[DK][2];
+        for (int x = 0; x < 2 * DK; ++x) {
+          const int q = lane + 32 * x, r = q / (4 * DK), c = q - r * 4 * DK;
+          const bool on = at >= 0 && (FULL || c * 16 < d);
+          cp_async16(to + k_at<DK>(r, c), kp + (FULL || on ? r * d + c * 16 : 0), on);
+        }
+#pragma unroll
+        for (int x = 0; x < VC / 4; ++x) {
+          const int q = lane + 32 * x, r = q / (VC / 2), c = q - r * (VC / 2);
+          const bool on = at >= 0 && (FULL || c * 16 < dv);
+          cp_async16(to + 16 * Cfg::KP + v_at<VC>(r, c), vp + (FULL || on ? r * dv + c * 16 : 0), on);
+        }
+      }
+      if ((i & 15) == 0) look_up_scale(2 * i);
+    }
+    cp_async_commit();
+  };
+
+  float f[NT][2], m[NT][2], l[NT][2], o[NT][MT][4];      // of the lane's columns 2t, 2t + 1
+
+  // The sums of the warps joined (common maximum, scaled sums in warp order) and written: the item's result, or this CTA's
+  // part of it.  `free`: the stage of the segment's last block, where every warp puts its O.
+  auto join = [&](const KvSegment& s, int free) {
+    float* s_o = reinterpret_cast<float*>(smem + (size_t)free * Cfg::STAGE);          // of warp 0
+    constexpr int WARP_O = STAGES * Cfg::STAGE / 4;                                    // floats from one warp's to the next
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], x);
+        if (g == 0) {
+          s_m[warp * ROWS + nt * 8 + 2 * t + j] = m[nt][j];
+          s_l[warp * ROWS + nt * 8 + 2 * t + j] = l[nt][j];
+        }
+      }
+    __syncthreads();
+    const bool whole = s.u0 == 0 && s.u1 == s.units;
+    const int slot = 2 * blockIdx.x + (s.u0 > 0 ? 0 : 1);
+#pragma unroll
+    for (int pass = 0; pass < NT / JOIN; ++pass) {
+      if (pass) __syncthreads();                           // O of the pass before has been read
+#pragma unroll
+      for (int n = 0; n < JOIN; ++n) {
+        const int nt = pass * JOIN + n;
+        float w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < KV_WARPS; ++x) top = fmaxf(top, s_m[x * ROWS + nt * 8 + 2 * t + j]);
+          w[j] = m[nt][j] == -INFINITY ? (l[nt][j] == 0.f ? 0.f : 1.f) : fast_exp2(m[nt][j] - top);    // (l NaN without a maximum: kept)
+        }
+#pragma unroll
+        for (int jj = 0; jj < MT; ++jj)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s_o[warp * WARP_O + ((n * MT + jj) * 4 + c) * 32 + lane] = o[nt][jj][c] * w[c & 1];
+      }
+      __syncthreads();
+      // thread = 4 neighbouring dims of a row
+#pragma unroll 1
+      for (int x = tid; x < JOIN * 8 * DV / 4; x += KV_WARPS * 32) {
+        constexpr int CH = VC < 16 ? VC : 16;              // bytes of one chunk
+        const int c8 = x / (DV / 4), dim = (x - c8 * (DV / 4)) * 4, chunk = dim / (8 * CH), in = dim - chunk * 8 * CH;
+        const int gg = in / CH, byte = in - gg * CH + chunk * CH, col = pass * JOIN * 8 + c8, row = s.row0 + col, i = row / p.G;
+        if (i >= p.S) continue;
+        const float* src = s_o + ((c8 >> 3) * MT * 4 + (byte >> 1) * 4 + (c8 & 1)) * 32 + gg * 4 + ((c8 & 7) >> 1);
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < KV_WARPS; ++k) {
+          top = fmaxf(top, s_m[k * ROWS + col]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] += src[k * WARP_O + (c >> 1) * 128 + (c & 1) * 64];
+        }
+#pragma unroll
+        for (int k = 0; k < KV_WARPS; ++k) {
+          const float mk = s_m[k * ROWS + col], lk = s_l[k * ROWS + col];
+          sum += mk == -INFINITY ? lk : lk * fast_exp2(mk - top);
+        }
+        if (whole) {
+          const int hq = s.h * p.G + row - i * p.G;
+          if (p.sink) {
+            const float sk = p.sink[hq] * kLog2e, up = fmaxf(top, sk), z = top == -INFINITY ? 1.f : fast_exp2(top - up);
+            sum = sum * z + (sk == -INFINITY ? 0.f : fast_exp2(sk - up));
+            v[0] *= z; v[1] *= z; v[2] *= z; v[3] *= z;
+            top = up;
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          if (dim == 0) p.lse[((int64_t)s.b * p.Hq + hq) * p.S + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+          if (FULL || dim < dv) {
+            const uint2 z = p.bf16 ? make_uint2(pack2<true>(v[0] * inv, v[1] * inv), pack2<true>(v[2] * inv, v[3] * inv))
+                                   : make_uint2(pack2<false>(v[0] * inv, v[1] * inv), pack2<false>(v[2] * inv, v[3] * inv));
+            *reinterpret_cast<uint2*>(p.o + (((int64_t)s.b * p.S + i) * p.Hq + hq) * dv + dim) = z;
+          }
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * ROWS + col) * DV + dim) = make_float4(v[0], v[1], v[2], v[3]);
+          if (dim == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * ROWS + col) * 2) = make_float2(top, sum);
+        }
+      }
+    }
+  };
+
+  KvSegment seg;
+  int seg_end = 0, lo_max = 0, hi_min = 0, stage = 0, free_stage = 0;
+#pragma unroll 1
+  for (int i = 1 - STAGES; i <= n_units; ++i) {
+    if (i >= 0 && i < n_units) {
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();                                    // block i is here, and every lane is done with block i - 1
+    }
+    const bool turn = i == seg_end;
+    KvSegment last;
+    uint4 x[DK][2];
+    if (turn) {
+      // the next item's queries (row g of tile `warp`) are on their way while the last one's sums are joined
+      last = seg;
+      if (i < n_units) seg = segment(u_begin + i);
+      const int row = seg.row0 + warp * 8 + g, qi = row / p.G;
+      const bool on = warp < NT && i < n_units && qi < p.S;
+      const uint16_t* src = p.q + seg.b * p.qs[0] + qi * p.qs[1] + ((int64_t)seg.h * p.G + row - qi * p.G) * p.qs[2];
 #pragma unroll
       for (int c = 0; c < DK; ++c)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int at = (t + 4 * c) * 16 + j * 8;
           x[c][j] = make_uint4(0, 0, 0, 0);
-          if (on && at < p.d) x[c][j] = __ldg(reinterpret_cast<const uint4*>(src + at));
+          if (on && (FULL || at < d)) x[c][j] = __ldg(reinterpret_cast<const uint4*>(src + at));
         }
-      float row_scale = 1.f;
-      if (p.bf16) {
-        // largest exponent of the row; fp16 then holds q 2^-e to 2^-24 of the row's largest value
-        uint32_t mx = 0;
-#pragma unroll
-        for (int c = 0; c < DK; ++c)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            mx = __vmaxu2(mx, x[c][j].x & 0x7f807f80u); mx = __vmaxu2(mx, x[c][j].y & 0x7f807f80u);
-            mx = __vmaxu2(mx, x[c][j].z & 0x7f807f80u); mx = __vmaxu2(mx, x[c][j].w & 0x7f807f80u);
-          }
-        mx = max(mx & 0xffffu, mx >> 16);
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = min(max((int)(mx >> 7), 1), 253);
-        row_scale = __uint_as_float((uint32_t)e << 23);
-        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-        for (int c = 0; c < DK; ++c)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&x[c][j]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) { const float2 v = unpack2<true>(w[q]); w[q] = pack2<false>(v.x * inv, v.y * inv); }
-          }
+      if (i > 0) join(last, free_stage);
+      if (i == n_units) break;
+      if (i > 0) __syncthreads();                          // the join's reads of O, m and l
+    }
+    fetch(i + STAGES - 1, free_stage);
+    free_stage = free_stage + 1 == STAGES ? 0 : free_stage + 1;
+    if (i < 0) continue;
+    if (turn) {
+      seg_end = i + seg.u1 - seg.u0;
+      if (tid < ROWS) {
+        const int row = (seg.row0 + tid) / p.G;
+        int lo, hi;
+        row_range(p, seg.r, row, lo, hi);
+        if (row >= p.S) { lo = 0; hi = INT_MAX; }          // (a column of zeros that nobody reads)
+        s_lim[tid] = make_int2(lo, hi);
       }
+      if (warp < NT) {
+        // bf16 -> fp16: the row's largest exponent goes into its scale, and fp16 holds q 2^-e to 2^-24 of the row's largest value
+        float scale = 1.f;
+        if (p.bf16) {
+          uint32_t mx = 0;
 #pragma unroll
-      for (int c = 0; c < DK; ++c) {
-        qf[nt][c][0][0] = x[c][0].x; qf[nt][c][0][1] = x[c][0].y; qf[nt][c][1][0] = x[c][0].z; qf[nt][c][1][1] = x[c][0].w;
-        qf[nt][c][2][0] = x[c][1].x; qf[nt][c][2][1] = x[c][1].y; qf[nt][c][3][0] = x[c][1].z; qf[nt][c][3][1] = x[c][1].w;
+          for (int c = 0; c < DK; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              mx = __vmaxu2(mx, x[c][j].x & 0x7f807f80u); mx = __vmaxu2(mx, x[c][j].y & 0x7f807f80u);
+              mx = __vmaxu2(mx, x[c][j].z & 0x7f807f80u); mx = __vmaxu2(mx, x[c][j].w & 0x7f807f80u);
+            }
+          mx = max(mx & 0xffffu, mx >> 16);
+          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const int e = min(max((int)(mx >> 7), 1), 253);
+          const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+          scale = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+          for (int c = 0; c < DK; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(&x[c][j]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) { const float2 v = unpack2<true>(w[q]); w[q] = pack2<false>(v.x * inv, v.y * inv); }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < DK; ++c) {
+          uint2* to = s_q + ((warp * DK + c) * 4) * 32 + lane;
+          to[0] = make_uint2(x[c][0].x, x[c][0].y); to[32] = make_uint2(x[c][0].z, x[c][0].w);
+          to[64] = make_uint2(x[c][1].x, x[c][1].y); to[96] = make_uint2(x[c][1].z, x[c][1].w);
+        }
+        if (t == 0) s_f[warp * 8 + g] = scale * p.scale_log2;
       }
+      __syncthreads();                                    // s_lim, s_q, s_f
+      lo_max = 0; hi_min = INT_MAX;
+      if (lane < ROWS) { lo_max = s_lim[lane].x; hi_min = s_lim[lane].y; }
+      lo_max = __reduce_max_sync(0xffffffffu, lo_max);
+      hi_min = __reduce_min_sync(0xffffffffu, hi_min);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f[nt][j] = __shfl_sync(0xffffffffu, row_scale, (2 * t + j) * 4) * p.scale_log2;
-        m[nt][j] = -INFINITY;
-        l[nt][j] = 0.f;
-        const int rj = row0 + nt * 8 + 2 * t + j, ij = rj / p.G;
-        row_range(p, r, ij, lo[nt][j], hi[nt][j]);
-        if (ij >= p.S) { lo[nt][j] = 0; hi[nt][j] = INT_MAX; }      // (a column of zeros that nobody reads)
-        lo_max = max(lo_max, lo[nt][j]);
-        hi_min = min(hi_min, hi[nt][j]);
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { f[nt][j] = s_f[nt * 8 + 2 * t + j]; m[nt][j] = -INFINITY; l[nt][j] = 0.f; }
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
       }
     }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      lo_max = max(lo_max, __shfl_xor_sync(0xffffffffu, lo_max, o));
-      hi_min = min(hi_min, __shfl_xor_sync(0xffffffffu, hi_min, o));
-    }
-    float o[NT][MT][4];
+    const uint32_t from = ring + stage * Cfg::STAGE;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    const int k0 = seg.key0 + KV_BLOCK * warp + (i - seg_end + seg.u1 - seg.u0) * KV_UNIT;
+
+    float s[NT][2][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < MT; ++j)
+      for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
-
-    // the warp's groups of 16 keys: key0 + 16 warp, then every KV_UNIT; their pages are looked up 32 at a time
-    const int n_groups = key1 > key0 + 16 * warp ? (key1 - key0 - 16 * warp + KV_UNIT - 1) / KV_UNIT : 0;
-    int my_page = -1;
-    float my_ks = 0.f, my_vs = 1.f;
-    auto look_up = [&](int first) {
-      const int i = first + lane;
-      my_page = i < n_groups ? kv_page(p.g, trow, key0 + 16 * warp + i * KV_UNIT) : -1;
-      if (my_page >= 0) {
-        my_ks = __ldg(p.ks + (size_t)my_page * p.g.Hkv + h);
-        my_vs = __ldg(p.vs + (size_t)my_page * p.g.Hkv + h);
-      }
-    };
-    uint4 kr[DK][2];
-    uint32_t vr[4][VW];
-    float ks = 0.f, vs = 1.f;
-    int page = -1;
-    auto fetch = [&](int i) {
-      if ((i & 31) == 0) look_up(i);
-      page = __shfl_sync(0xffffffffu, my_page, i & 31);
-      ks = __shfl_sync(0xffffffffu, my_ks, i & 31);
-      vs = __shfl_sync(0xffffffffu, my_vs, i & 31);
-      if (page < 0) return;
-      const int slot = (key0 + 16 * warp + i * KV_UNIT) & ((1 << p.g.page_log2) - 1);
-      const size_t at = (((size_t)page * p.g.Hkv + h) << p.g.page_log2) + slot;
-      const uint8_t* kp = p.k + (at + g) * p.d + t * 16;
+        for (int c = 0; c < 4; ++c) s[nt][hh][c] = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < DK; ++c) {
+      uint4 x[2][2];
 #pragma unroll
-      for (int c = 0; c < DK; ++c) {
-        const bool on = (t + 4 * c) * 16 < p.d;
-        kr[c][0] = on ? ldg_stream(kp + c * 64) : make_uint4(0, 0, 0, 0);
-        kr[c][1] = on ? ldg_stream(kp + c * 64 + 8 * p.d) : make_uint4(0, 0, 0, 0);
+      for (int hh = 0; hh < 2; ++hh) {
+        x[hh][0] = lds128(from + hh * Cfg::GROUP + k_at<DK>(g, t + 4 * c));
+        x[hh][1] = lds128(from + hh * Cfg::GROUP + k_at<DK>(g + 8, t + 4 * c));
       }
-      const uint8_t* vp = p.v + (at + 2 * t) * p.dv + g * (VC < 16 ? VC : 16);
+      const uint2* q = s_q + c * 128 + lane;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t fr[2][4];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const uint32_t a = j == 0 ? x[hh][0].x : (j == 1 ? x[hh][0].y : (j == 2 ? x[hh][0].z : x[hh][0].w));
+          const uint32_t z = j == 0 ? x[hh][1].x : (j == 1 ? x[hh][1].y : (j == 2 ? x[hh][1].z : x[hh][1].w));
+          from_payload4<INT8>(a, fr[hh][0], fr[hh][2]);
+          from_payload4<INT8>(z, fr[hh][1], fr[hh][3]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint2 y = q[nt * DK * 128 + j * 32];
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) mma16816<false>(s[nt][hh], fr[hh], y.x, y.y);
+        }
+      }
+    }
+    const float4 i0 = info[(2 * i) & (KV_INFO - 1)], i1 = info[(2 * i + 1) & (KV_INFO - 1)];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float a = f[nt][j] * i0.x, z = f[nt][j] * i1.x;
+        s[nt][0][j] = s[nt][0][j] * a + i0.y; s[nt][0][2 + j] = s[nt][0][2 + j] * a + i0.y;
+        s[nt][1][j] = s[nt][1][j] * z + i1.y; s[nt][1][2 + j] = s[nt][1][2 + j] * z + i1.y;
+      }
+    uint32_t hidden = 0;                                   // bit nt * 8 + hh * 4 + q of a score that its row does not see
+    const bool cut = k0 < lo_max || k0 + KV_BLOCK > hi_min;
+    if (cut) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int2 lim = s_lim[nt * 8 + 2 * t + j];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int key = k0 + g + 8 * q;
+            if (key < lim.x || key >= lim.y) {
+              s[nt][q >> 1][(q & 1) * 2 + j] = -INFINITY;
+              hidden |= 1u << (nt * 8 + (q >> 1) * 4 + (q & 1) * 2 + j);
+            }
+          }
+        }
+    }
+    bool grow = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        grow |= fmaxf(fmax3(s[nt][0][j], s[nt][0][2 + j], s[nt][1][j]), s[nt][1][2 + j]) > m[nt][j] + 15.f;
+    // m is kept 7 below the running maximum and lags: it moves where a score is more than 15 above it.  p is at most 2^15, and
+    // fp16 keeps its relative precision down to 2^-21 of the largest
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x = fmaxf(fmax3(s[nt][0][j], s[nt][0][2 + j], s[nt][1][j]), s[nt][1][2 + j]);
+#pragma unroll
+          for (int y = 4; y < 32; y <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
+          x = fmaxf(x - 7.f, m[nt][j]);
+          const float w = x == -INFINITY ? 1.f : fast_exp2(m[nt][j] - x);
+          m[nt][j] = x;
+          l[nt][j] *= w;
+#pragma unroll
+          for (int jj = 0; jj < MT; ++jj) { o[nt][jj][j] *= w; o[nt][jj][2 + j] *= w; }
+        }
+    }
+    uint32_t pb[2][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        float e[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) e[q] = fast_exp2(s[nt][hh][q] - (q & 1 ? m1 : m0));
+        l[nt][0] += (e[0] + e[2]) * (hh ? i1.z : i0.z);
+        l[nt][1] += (e[1] + e[3]) * (hh ? i1.z : i0.z);
+        pb[hh][nt][0] = movmatrix_trans(pack2<false>(e[0], e[1]));
+        pb[hh][nt][1] = movmatrix_trans(pack2<false>(e[2], e[3]));
+      }
+    }
+#pragma unroll 1
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t vc[4][VW];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const uint8_t* q = vp + ((x & 1) + (x >> 1) * 8) * p.dv;
+        const int r = 2 * t + (x & 1) + (x >> 1) * 8;
+        const uint32_t at = from + hh * Cfg::GROUP + 16 * Cfg::KP;
         if constexpr (VC == 8) {
-          uint2 v = make_uint2(0, 0);
-          if (g * 8 < p.dv) v = __ldg(reinterpret_cast<const uint2*>(q));
-          vr[x][0] = v.x; vr[x][1] = v.y;
+          const uint2 v = lds64(at + v_at<VC>(r, g >> 1) + (g & 1) * 8);
+          vc[x][0] = v.x; vc[x][1] = v.y;
         } else {
 #pragma unroll
           for (int c = 0; c < VC / 16; ++c) {
-            const uint4 v = g * 16 + c * 128 < p.dv ? ldg_stream(q + c * 128) : make_uint4(0, 0, 0, 0);
-            vr[x][4 * c] = v.x; vr[x][4 * c + 1] = v.y; vr[x][4 * c + 2] = v.z; vr[x][4 * c + 3] = v.w;
+            const uint4 v = lds128(at + v_at<VC>(r, g + 8 * c));
+            vc[x][4 * c] = v.x; vc[x][4 * c + 1] = v.y; vc[x][4 * c + 2] = v.z; vc[x][4 * c + 3] = v.w;
           }
         }
       }
-    };
-    if (n_groups) fetch(0);
-    for (int i = 0; i < n_groups; ++i) {
-      // this group's payload out of the way of the next one's
-      uint4 kc[DK][2];
-      uint32_t vc[4][VW];
-#pragma unroll
-      for (int c = 0; c < DK; ++c) { kc[c][0] = kr[c][0]; kc[c][1] = kr[c][1]; }
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int c = 0; c < VW; ++c) vc[x][c] = vr[x][c];
-      const float ks_now = ks, vs_now = vs;
-      const bool no_page = page < 0;
-      const int k0 = key0 + 16 * warp + i * KV_UNIT;
-      if (i + 1 < n_groups) fetch(i + 1);
-      if (no_page) continue;
-
-      float s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[nt][c] = 0.f;
-#pragma unroll
-      for (int c = 0; c < DK; ++c) {
-        const uint32_t a[4] = {kc[c][0].x, kc[c][0].y, kc[c][0].z, kc[c][0].w}, z[4] = {kc[c][1].x, kc[c][1].y, kc[c][1].z, kc[c][1].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t fr[4];
-          from_payload4<INT8>(a[j], fr[0], fr[2]);
-          from_payload4<INT8>(z[j], fr[1], fr[3]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<false>(s[nt], fr, qf[nt][c][j][0], qf[nt][c][j][1]);
-        }
-      }
-      // (a NaN scale: the scores of the keys that are seen carry it)
-      const float lv = log2f(vs_now), inv_vs = vs_now > 0.f ? 1.f / vs_now : 1.f;
-      const bool cut = k0 < lo_max || k0 + 16 > hi_min;
-      bool grow = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float fk = f[nt][j] * ks_now;
-          float x = s[nt][j] * fk + lv, y = s[nt][2 + j] * fk + lv;
-          if (cut) {
-            if (k0 + g < lo[nt][j] || k0 + g >= hi[nt][j]) x = -INFINITY;
-            if (k0 + g + 8 < lo[nt][j] || k0 + g + 8 >= hi[nt][j]) y = -INFINITY;
-          }
-          s[nt][j] = x; s[nt][2 + j] = y;
-          grow |= fmaxf(x, y) > m[nt][j] + 8.f;
-        }
-      // the running maximum lags: it moves where a score is more than 2^8 above it
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float x = fmaxf(s[nt][j], s[nt][2 + j]);
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            x = fmaxf(x, m[nt][j]);
-            const float w = x == -INFINITY ? 1.f : fast_exp2(m[nt][j] - x);
-            m[nt][j] = x;
-            l[nt][j] *= w;
-#pragma unroll
-            for (int jj = 0; jj < MT; ++jj) { o[nt][jj][j] *= w; o[nt][jj][2 + j] *= w; }
-          }
-      }
-      uint32_t pb[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float e[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float mm = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-          e[j] = fast_exp2(s[nt][j] - mm);
-          e[2 + j] = fast_exp2(s[nt][2 + j] - mm);
-          l[nt][j] += (e[j] + e[2 + j]) * inv_vs;
-        }
-        pb[nt][0] = movmatrix_trans(pack2<false>(e[0], e[1]));
-        pb[nt][1] = movmatrix_trans(pack2<false>(e[2], e[3]));
-      }
-      if constexpr (!INT8) {
+      if (!INT8 && cut) {
         // A NaN among values that a row does not see (slots behind the sequence hold whatever was there) must stay out of
-        // that row, and 0 * NaN would not: where a group that some row sees in part holds one, the NaNs are multiplied
+        // that row, and 0 * NaN would not: where a block that some row sees in part holds one, the NaNs are multiplied
         // apart, as ones, with what every row sees.
         uint32_t found = 0;
-        if (cut)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int c = 0; c < VW; ++c) found |= nan_bytes(vc[x][c]);
+          for (int c = 0; c < VW; ++c) found |= nan_bytes(vc[x][c]);
         if (__any_sync(0xffffffffu, found != 0)) {
-          uint32_t sb[NT][2];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float w[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) w[q] = s[nt][q] == -INFINITY ? 0.f : 1.f;
-            sb[nt][0] = movmatrix_trans(pack2<false>(w[0], w[1]));
-            sb[nt][1] = movmatrix_trans(pack2<false>(w[2], w[3]));
-          }
 #pragma unroll
           for (int c = 0; c < VW; ++c) {
             uint32_t bad[4];
@@ -366,8 +555,10 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) kv_attn_kernel(const KvAttnP
               from_payload4<INT8>(__byte_perm(bad[2], bad[3], sel), fr[2], fr[3]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                float seen[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816<false>(seen, fr, sb[nt][0], sb[nt][1]);
+                float w[4], seen[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) w[q] = hidden >> (nt * 8 + hh * 4 + q) & 1u ? 0.f : 1.f;
+                mma16816<false>(seen, fr, movmatrix_trans(pack2<false>(w[0], w[1])), movmatrix_trans(pack2<false>(w[2], w[3])));
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                   if (seen[q] > 0.f) o[nt][2 * c + half][q] = __uint_as_float(0x7fffffffu);
@@ -385,150 +576,101 @@ __global__ void __launch_bounds__(KV_WARPS * 32, 1) kv_attn_kernel(const KvAttnP
           from_payload4<INT8>(__byte_perm(vc[0][c], vc[1][c], sel), fr[0], fr[1]);
           from_payload4<INT8>(__byte_perm(vc[2][c], vc[3][c], sel), fr[2], fr[3]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][2 * c + half], fr, pb[nt][0], pb[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][2 * c + half], fr, pb[0][nt][0], pb[0][nt][1]);
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) { pb[0][nt][0] = pb[1][nt][0]; pb[0][nt][1] = pb[1][nt][1]; }
     }
-
-    // join the warps: common maximum, scaled sums in warp order
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
-        if (g == 0) {
-          s_m[warp * ROWS + nt * 8 + 2 * t + j] = m[nt][j];
-          s_l[warp * ROWS + nt * 8 + 2 * t + j] = l[nt][j];
-        }
-      }
-    __syncthreads();
-    const bool whole = u0 == 0 && u1 == units;
-    const int slot = 2 * blockIdx.x + (u0 > 0 ? 0 : 1);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int col = nt * 8 + 2 * t + j;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < KV_WARPS; ++w) top = fmaxf(top, s_m[w * ROWS + col]);
-        const float w = m[nt][j] == -INFINITY ? (l[nt][j] == 0.f ? 0.f : 1.f) : fast_exp2(m[nt][j] - top);    // (l NaN without a maximum: kept)
-#pragma unroll
-        for (int jj = 0; jj < MT; ++jj) {
-          s_o[(warp * MT * 4 + jj * 4 + j) * 32 + lane] = o[nt][jj][j] * w;
-          s_o[(warp * MT * 4 + jj * 4 + 2 + j) * 32 + lane] = o[nt][jj][2 + j] * w;
-        }
-      }
-      __syncthreads();
-      // thread = 4 neighbouring dims of a row
-      for (int x = tid; x < 8 * DV / 4; x += KV_WARPS * 32) {
-        const int col = x / (DV / 4), dim = (x - col * (DV / 4)) * 4, row = row0 + nt * 8 + col, i = row / p.G;
-        constexpr int CH = VC < 16 ? VC : 16;              // bytes of one chunk
-        const int chunk = dim / (8 * CH), in = dim - chunk * 8 * CH, gg = in / CH, byte = in - gg * CH + chunk * CH;
-        float v[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < KV_WARPS; ++w) {
-          top = fmaxf(top, s_m[w * ROWS + nt * 8 + col]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            v[c] += s_o[(w * MT * 4 + ((byte + c) >> 1) * 4 + ((byte + c) & 1) * 2 + (col & 1)) * 32 + gg * 4 + (col >> 1)];
-        }
-#pragma unroll
-        for (int w = 0; w < KV_WARPS; ++w) {
-          const float mw = s_m[w * ROWS + nt * 8 + col], lw = s_l[w * ROWS + nt * 8 + col];
-          sum += mw == -INFINITY ? lw : lw * fast_exp2(mw - top);
-        }
-        if (i >= p.S) continue;
-        if (whole) {
-          const int hq = h * p.G + row - i * p.G;
-          const float sk = p.sink ? p.sink[hq] * kLog2e : -INFINITY;
-          if (p.sink) {
-            const float up = fmaxf(top, sk), w = top == -INFINITY ? 1.f : fast_exp2(top - up);
-            sum = sum * w + (sk == -INFINITY ? 0.f : fast_exp2(sk - up));
-            v[0] *= w; v[1] *= w; v[2] *= w; v[3] *= w;
-            top = up;
-          }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          if (dim == 0) p.lse[((int64_t)b * p.Hq + hq) * p.S + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-          if (dim < p.dv) {
-            const uint2 w = p.bf16 ? make_uint2(pack2<true>(v[0] * inv, v[1] * inv), pack2<true>(v[2] * inv, v[3] * inv))
-                                   : make_uint2(pack2<false>(v[0] * inv, v[1] * inv), pack2<false>(v[2] * inv, v[3] * inv));
-            *reinterpret_cast<uint2*>(p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * p.dv + dim) = w;
-          }
-        } else {
-          *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * ROWS + nt * 8 + col) * DV + dim) = make_float4(v[0], v[1], v[2], v[3]);
-          if (dim == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * ROWS + nt * 8 + col) * 2) = make_float2(top, sum);
-        }
-      }
-      __syncthreads();
-    }
-    u_at += u1 - u0;
   }
-  grid_dep_trigger();
 }
 
-// One CTA = one query row (of a kv head's rows) of one item that was cut: its parts lie in consecutive CTAs' slots.
-// Four groups of 32 lanes take the parts in turn and are then joined in order.
+// One CTA = one query row (of a kv head's rows) of one item; it joins the parts when the item was cut, which lie in
+// consecutive CTAs' slots.  Where the item was cut follows from the lengths, which are there before the parts are.  Every
+// warp computes all parts' weights, a lane each; the warps take the parts in turn and are joined in order.
 template <int DV, int ROWS>
 __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p) {
-  constexpr int PER = DV / 32;
-  __shared__ float s_v[4][DV], s_m[4], s_l[4];
-  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, b = blockIdx.z, h = blockIdx.y, row = blockIdx.x;
-  grid_dep_wait();
-  const int64_t total = p.pre[p.B], n = p.n_cta;
-  const int first = p.pre[b], units = (p.pre[b + 1] - first) / (p.g.Hkv * p.row_tiles), tile = row / ROWS;
-  const int64_t s0 = first + (int64_t)(h * p.row_tiles + tile) * units, s1 = s0 + units - 1;
-  const int c0 = (int)(((s0 + 1) * n - 1) / total), c1 = (int)(((s1 + 1) * n - 1) / total);
-  if (c0 == c1) return;                                   // done by one CTA
-  float m = -INFINITY, l = 0.f, v[PER];
-#pragma unroll
-  for (int x = 0; x < PER; ++x) v[x] = 0.f;
-  for (int c = c0 + grp; c <= c1; c += 4) {
-    const size_t at = (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS + row - tile * ROWS;
-    // (no unit of the item in this CTA: an empty range, as with fewer units than CTAs)
-    if (total * (c + 1) / n == total * c / n) continue;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-    float y[PER];
-    if constexpr (PER == 2) { const float2 q = *reinterpret_cast<const float2*>(p.part_o + at * DV + lane * 2); y[0] = q.x; y[1] = q.y; }
-    else
-#pragma unroll
-      for (int x = 0; x < PER; x += 4) {
-        const float4 q = *reinterpret_cast<const float4*>(p.part_o + at * DV + lane * PER + x);
-        y[x] = q.x; y[x + 1] = q.y; y[x + 2] = q.z; y[x + 3] = q.w;
-      }
-    const float top = fmaxf(m, ml.x), w0 = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - top),
-                w1 = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);
-    l = l * w0 + ml.y * w1;
-    m = top;
-#pragma unroll
-    for (int x = 0; x < PER; ++x) v[x] = v[x] * w0 + y[x] * w1;
+  constexpr int PER = DV / 32, AHEAD = 4;
+  __shared__ float s_v[4][DV];
+  __shared__ int s_sum[2][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, h = blockIdx.y, row = blockIdx.x;
+  const int items = p.g.Hkv * p.row_tiles, mine = kv_units(kv_range(p, b));
+  int before = 0, all = 0;
+  for (int x = threadIdx.x; x < p.B; x += 128) {
+    const int n = kv_units(kv_range(p, x)) * items;
+    all += n;
+    before += x < b ? n : 0;
   }
 #pragma unroll
-  for (int x = 0; x < PER; ++x) s_v[grp][lane * PER + x] = v[x];
-  if (lane == 0) { s_m[grp] = m; s_l[grp] = l; }
+  for (int o = 16; o; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); }
+  if (lane == 0) { s_sum[0][warp] = all; s_sum[1][warp] = before; }
   __syncthreads();
+  const int64_t total = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3], n = min((int64_t)p.n_cta, total);
+  before = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
+  const int tile = row / ROWS, in_tile = row - tile * ROWS;
+  const int64_t s0 = before + (int64_t)(h * p.row_tiles + tile) * mine, s1 = s0 + mine - 1;
+  const int c0 = (int)(((s0 + 1) * n - 1) / total), c1 = (int)(((s1 + 1) * n - 1) / total);
+  grid_dep_wait();
+  if (c0 == c1) return;                                   // done by one CTA
+  auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS + in_tile; };
+  auto get_ml = [&](int c) {
+    return c <= c1 ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot(c)) : make_float2(-INFINITY, 0.f);
+  };
+  float y[AHEAD][PER];
+  auto get_o = [&](int c) {                              // AHEAD parts of this warp, from c on
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const float* src = p.part_o + slot(c + 4 * a) * DV + lane * PER;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) y[a][e] = 0.f;
+      if (c + 4 * a > c1) continue;
+      if constexpr (PER == 2) { const float2 q = __ldcg(reinterpret_cast<const float2*>(src)); y[a][0] = q.x; y[a][1] = q.y; }
+      else {
+#pragma unroll
+        for (int e = 0; e < PER; e += 4) {
+          const float4 q = __ldcg(reinterpret_cast<const float4*>(src + e));
+          y[a][e] = q.x; y[a][e + 1] = q.y; y[a][e + 2] = q.z; y[a][e + 3] = q.w;
+        }
+      }
+    }
+  };
+  float2 ml = get_ml(c0 + lane);
+  get_o(c0 + warp);
   const int i = row / p.G, hq = h * p.G + row - i * p.G;
   const float sk = p.sink ? p.sink[hq] * kLog2e : -INFINITY;
-  float top = sk;
+  float top = fmaxf(sk, ml.x);
+  for (int c = c0 + 32 + lane; c <= c1; c += 32) top = fmaxf(top, get_ml(c).x);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) top = fmaxf(top, s_m[q]);
-  float w[4], sum = sk == -INFINITY ? 0.f : fast_exp2(sk - top);
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f, v[PER];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    w[q] = s_m[q] == -INFINITY ? (s_l[q] == 0.f ? 0.f : 1.f) : fast_exp2(s_m[q] - top);
-    sum += s_l[q] * w[q];
+  for (int x = 0; x < PER; ++x) v[x] = 0.f;
+  for (int base = c0; base <= c1; base += 32) {
+    if (base > c0) ml = get_ml(base + lane);
+    const float w_mine = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);    // (l NaN without a maximum: kept)
+    sum += ml.y * w_mine;
+    for (int x0 = warp; x0 < 32 && base + x0 <= c1; x0 += 4 * AHEAD) {
+      if (base + x0 > c0 + warp) get_o(base + x0);
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const float w = __shfl_sync(0xffffffffu, w_mine, x0 + 4 * a);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) v[e] += base + x0 + 4 * a <= c1 ? w * y[a][e] : 0.f;
+      }
+    }
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (sk != -INFINITY) sum += fast_exp2(sk - top);
+#pragma unroll
+  for (int x = 0; x < PER; ++x) s_v[warp][lane * PER + x] = v[x];
+  __syncthreads();
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (threadIdx.x == 0) p.lse[((int64_t)b * p.Hq + hq) * p.S + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-  for (int dim = threadIdx.x; dim < p.dv; dim += 128) {
-    float x = 0.f;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) x += s_v[q][dim] * w[q];
-    x *= inv;
-    const size_t at = (((int64_t)b * p.S + i) * p.Hq + hq) * p.dv + dim;
-    if (p.bf16) reinterpret_cast<__nv_bfloat16*>(p.o)[at] = __float2bfloat16_rn(x);
-    else reinterpret_cast<__half*>(p.o)[at] = __float2half_rn(x);
+  for (int dim = threadIdx.x * 2; dim < p.dv; dim += 256) {
+    const float x = (s_v[0][dim] + s_v[1][dim] + s_v[2][dim] + s_v[3][dim]) * inv;
+    const float y = (s_v[0][dim + 1] + s_v[1][dim + 1] + s_v[2][dim + 1] + s_v[3][dim + 1]) * inv;
+    *reinterpret_cast<uint32_t*>(p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * p.dv + dim) = p.bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
   }
 }
 
@@ -538,25 +680,27 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p
 int sm_count();
 int kv_geometry(const fm_kv_cache* c, const fm_kv_args* a, KvGeom* g);
 
-constexpr int KV_MAX_B = 8192;                      // first units of the sequences are kept in shared memory
+constexpr int KV_MAX_B = 1024;                      // first units of the sequences are kept in shared memory
 
-struct KvAttnPlan { int vc, nt, n_cta; size_t pre_bytes, bytes; };
+struct KvAttnPlan { int vc, nt, n_cta; size_t bytes; };
 static KvAttnPlan kv_attn_plan(const fm_kv_cache* c, const fm_kv_args* a) {
   KvAttnPlan pl;
   const int rows = a->S * (a->Hq / c->Hkv);
   pl.vc = c->dv <= 64 && c->d <= 64 ? 8 : (c->dv <= 128 ? 16 : 32);
-  pl.nt = rows <= 8 || pl.vc == 32 ? 1 : 2;
-  pl.n_cta = sm_count();
-  pl.pre_bytes = ((size_t)(a->B + 1) * sizeof(int) + 15) & ~(size_t)15;
-  pl.bytes = pl.pre_bytes + (size_t)2 * pl.n_cta * pl.nt * 8 * (8 * pl.vc + 2) * sizeof(float);
+  pl.nt = rows <= 8 || pl.vc == 32 ? 1 : (rows <= 16 || c->d > 128 ? 2 : 4);
+  pl.n_cta = sm_count() * (pl.vc > 16 ? KvCfg<4, 32, 1>::CTAS : c->d > 128 ? KvCfg<3, 16, 1>::CTAS
+             : pl.vc == 16 ? (pl.nt == 1 ? KvCfg<2, 16, 1>::CTAS : pl.nt == 2 ? KvCfg<2, 16, 2>::CTAS : KvCfg<2, 16, 4>::CTAS)
+                           : (pl.nt == 1 ? KvCfg<1, 8, 1>::CTAS : pl.nt == 2 ? KvCfg<1, 8, 2>::CTAS : KvCfg<1, 8, 4>::CTAS));
+  pl.bytes = (size_t)2 * pl.n_cta * pl.nt * 8 * (8 * pl.vc + 2) * sizeof(float);
   return pl;
 }
 
-template <int DK, int VC, int NT, bool INT8>
+template <int DK, int VC, int NT, bool INT8, bool FULL>
 static int launch_kv_attn(const KvAttnParams& p, cudaStream_t s) {
-  auto kern = kv_attn_kernel<DK, VC, NT, INT8>;
-  const size_t smem = (size_t)(KV_WARPS * (VC / 2) * 128 + 2 * KV_WARPS * 8 * NT + p.B + 1) * 4;
-  FM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+  using Cfg = KvCfg<DK, VC, NT>;
+  auto kern = kv_attn_kernel<DK, VC, NT, INT8, FULL>;
+  const size_t smem = Cfg::FIXED + (size_t)(p.B + 1) * 4;
+  FM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::FIXED + (KV_MAX_B + 1) * 4));
   kern<<<p.n_cta, KV_WARPS * 32, smem, s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
@@ -565,12 +709,22 @@ static int launch_kv_attn(const KvAttnParams& p, cudaStream_t s) {
   return FM_OK;
 }
 
+template <int DK, int VC, bool INT8, bool FULL>
+static int launch_kv_attn_rows(const KvAttnParams& p, int nt, cudaStream_t s) {
+  if (nt == 1 || VC > 16) return launch_kv_attn<DK, VC, 1, INT8, FULL>(p, s);
+  if constexpr (VC <= 16) {
+    if (nt == 2 || DK > 2) return launch_kv_attn<DK, VC, 2, INT8, FULL>(p, s);
+    if constexpr (DK <= 2) return launch_kv_attn<DK, VC, 4, INT8, FULL>(p, s);
+  }
+  return FM_ERR_UNSUPPORTED;
+}
+
 template <bool INT8>
 static int dispatch_kv_attn(const KvAttnParams& p, const KvAttnPlan& pl, cudaStream_t s) {
-  if (pl.vc == 32) return launch_kv_attn<4, 32, 1, INT8>(p, s);
-  if (p.d == 192) return pl.nt == 1 ? launch_kv_attn<3, 16, 1, INT8>(p, s) : launch_kv_attn<3, 16, 2, INT8>(p, s);
-  if (pl.vc == 16) return pl.nt == 1 ? launch_kv_attn<2, 16, 1, INT8>(p, s) : launch_kv_attn<2, 16, 2, INT8>(p, s);
-  return pl.nt == 1 ? launch_kv_attn<1, 8, 1, INT8>(p, s) : launch_kv_attn<1, 8, 2, INT8>(p, s);
+  if (pl.vc == 32) return launch_kv_attn_rows<4, 32, INT8, true>(p, pl.nt, s);
+  if (p.d == 192) return launch_kv_attn_rows<3, 16, INT8, true>(p, pl.nt, s);
+  if (pl.vc == 16) return p.d == 128 && p.dv == 128 ? launch_kv_attn_rows<2, 16, INT8, true>(p, pl.nt, s) : launch_kv_attn_rows<2, 16, INT8, false>(p, pl.nt, s);
+  return p.d == 64 && p.dv == 64 ? launch_kv_attn_rows<1, 8, INT8, true>(p, pl.nt, s) : launch_kv_attn_rows<1, 8, INT8, false>(p, pl.nt, s);
 }
 
 }  // namespace fm
@@ -603,6 +757,7 @@ extern "C" FM_API int fm_kv_attention(const fm_kv_cache* c, const fm_kv_args* a,
   const int64_t G = a->Hq / c->Hkv, rows = a->S * G, tiles = (rows + pl.nt * 8 - 1) / (pl.nt * 8);
   const int64_t units = ((int64_t)a->max_pages * c->page_size + 31) / KV_UNIT + 1;
   FM_REQUIRE(rows < INT_MAX && units * tiles <= (INT_MAX - 1) / c->Hkv / a->B, FM_ERR_UNSUPPORTED, "fm_kv_attention: too many rows and keys for one call");
+  FM_REQUIRE((int64_t)c->num_pages * c->Hkv * c->page_size / 16 < INT_MAX, FM_ERR_UNSUPPORTED, "fm_kv_attention: a cache of 2^31 groups of 16 tokens");
   FM_REQUIRE(a->workspace && a->workspace_bytes >= pl.bytes && ((uintptr_t)a->workspace & 15) == 0, FM_ERR_WORKSPACE,
              "fm_kv_attention: workspace of %zu bytes, %zu needed", a->workspace_bytes, pl.bytes);
   p.k = (const uint8_t*)c->k; p.v = (const uint8_t*)c->v; p.ks = c->k_scale; p.vs = c->v_scale;
@@ -613,8 +768,7 @@ extern "C" FM_API int fm_kv_attention(const fm_kv_cache* c, const fm_kv_args* a,
   p.row_tiles = (int)tiles;
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.n_cta = pl.n_cta;
-  p.pre = (int*)a->workspace;
-  p.part_o = (float*)((char*)a->workspace + pl.pre_bytes);
+  p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + (size_t)2 * pl.n_cta * pl.nt * 8 * 8 * pl.vc;
   return c->dtype == FM_CACHE_INT8 ? dispatch_kv_attn<true>(p, pl, (cudaStream_t)stream) : dispatch_kv_attn<false>(p, pl, (cudaStream_t)stream);
 }

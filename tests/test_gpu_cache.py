@@ -40,6 +40,11 @@ class Filled:
             getattr(self.cache, name + "_scale").copy_(scale.cuda())
         self.seqlens = torch.tensor(lens, dtype=torch.int32)
 
+    def largest_scale(self, b):
+        own = [p for p in self.table[b].tolist() if 0 <= p < self.cache.k.shape[0]]
+        s = self.cache.v_scale.cpu()[own]
+        return float(s[torch.isfinite(s)].max()) if len(own) else 0.0
+
     def dense(self, b, name, n=None):
         return ref.dense(values_of(getattr(self.cache, name)), getattr(self.cache, name + "_scale").cpu().double(), self.table[b],
                          self.lens[b] if n is None else n)
@@ -65,7 +70,9 @@ def check_attention(f, q, *, q_lengths=None, causal=True, window=None, scale=Non
         p_half = 2.0 ** -8 if S * Hq // f.cache.k.shape[1] > 64 and q.dtype == torch.bfloat16 else 2.0 ** -11
         slack = reach * (d + 16) * 2.0 ** -23 + 2.0 ** -20 + max(n, 1) * 2.0 ** -24
         # (below the smallest normal number of the type half a step is no longer relative: smallest normal * eps / 2, 2^-25 in fp16)
-        tol = half * o.abs() + weight * (p_half + 2 * slack[..., None]) + torch.finfo(q.dtype).smallest_normal * half
+        # (fp16's half step is 2^-25 for p below 2^-14, when the largest p is 2^7 at least: 2^-32 of the largest p_j vs_j for every
+        # payload value, at most 448; the dense forward in bf16 has the same relative step everywhere, in fp16 2^-25 of the largest p)
+        tol = half * o.abs() + n * 2.0 ** (-32 if S * Hq // f.cache.k.shape[1] <= 64 else -25) * 448 * f.largest_scale(b) + weight * (p_half + 2 * slack[..., None]) + torch.finfo(q.dtype).smallest_normal * half
         far = (out[b] - o).abs() - tol
         w = far.argmax()
         assert far.flatten()[w] <= 0, (b, int(w), *(t.flatten()[w].item() for t in (far, out[b], o, weight)))
