@@ -25,9 +25,18 @@ struct NormParams {
   const float* cos; const float* sin;                          // [table, rot / 2]
   const void* pos; int pos64; int64_t pos_b;                   // [B, S] with that batch stride, or NULL: the token's index
   int B, S, H[2], d, rot, table, w_f32;
-  int chunks, per_chunk;                                       // a token's groups of heads are dealt to `chunks` warps
-  float eps;
+  int chunks[2], per_chunk[2];                                 // a token's groups of 32 / LPR heads are dealt to `chunks` jobs
+  float eps, inv_d;
 };
+
+// Two fp32 lanes in a 64-bit register (sm_100 packed arithmetic): one instruction for two values.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pair(float a, float b) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void unpair(f2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ f2 mul(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f2 swap(f2 x) { float a, b; unpair(x, a, b); return pair(b, a); }
+__device__ __forceinline__ float sum(f2 x) { float a, b; unpair(x, a, b); return a + b; }
 
 // Offsets of the two vectors of 8 of slot `s` in a row.
 template <bool INTERLEAVED>
@@ -36,40 +45,56 @@ __device__ __forceinline__ void slot_offsets(int s, int rot, int& lo, int& hi) {
   else { lo = s * 8; hi = rot / 2 + lo; }
 }
 
+// A slot: v[0 .. 3] the first vector, v[4 .. 7] the second.
+struct Raw { uint4 lo, hi; };
 template <bool IS_BF16>
-__device__ __forceinline__ void load8(float (&v)[8], const uint16_t* p) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void widen(f2 (&v)[8], const Raw& r) {
+  const uint32_t w[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { const float2 f = unpack2<IS_BF16>(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+  for (int i = 0; i < 8; ++i) { const float2 f = unpack2<IS_BF16>(w[i]); v[i] = pair(f.x, f.y); }
 }
 template <bool IS_BF16>
-__device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack2<IS_BF16>(v[0], v[1]), pack2<IS_BF16>(v[2], v[3]), pack2<IS_BF16>(v[4], v[5]), pack2<IS_BF16>(v[6], v[7]));
+__device__ __forceinline__ uint32_t narrow(f2 x) { float a, b; unpair(x, a, b); return pack2<IS_BF16>(a, b); }
+template <bool IS_BF16>
+__device__ __forceinline__ void store(uint16_t* p, int lo, int hi, const f2 (&v)[8]) {
+  *reinterpret_cast<uint4*>(p + lo) = make_uint4(narrow<IS_BF16>(v[0]), narrow<IS_BF16>(v[1]), narrow<IS_BF16>(v[2]), narrow<IS_BF16>(v[3]));
+  *reinterpret_cast<uint4*>(p + hi) = make_uint4(narrow<IS_BF16>(v[4]), narrow<IS_BF16>(v[5]), narrow<IS_BF16>(v[6]), narrow<IS_BF16>(v[7]));
 }
 template <bool IS_BF16>
-__device__ __forceinline__ void load_weight8(float (&v)[8], const void* w, int w_f32, int at) {
+__device__ __forceinline__ void load_weight(f2 (&v)[8], const void* w, int w_f32, int lo, int hi) {
   if (!w) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 1.f;
+    for (int i = 0; i < 8; ++i) v[i] = pair(1.f, 1.f);
   } else if (w_f32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __ldg(reinterpret_cast<const float*>(w) + at + i);
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(w) + (i < 4 ? lo + 2 * i : hi + 2 * i - 8)));
+      v[i] = pair(f.x, f.y);
+    }
   } else {
-    load8<IS_BF16>(v, reinterpret_cast<const uint16_t*>(w) + at);
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(w);
+    widen<IS_BF16>(v, Raw{__ldg(reinterpret_cast<const uint4*>(p + lo)), __ldg(reinterpret_cast<const uint4*>(p + hi))});
   }
 }
 
-// Turns the 8 pairs of a slot by the angles (c, s), or by minus them.
+// Turns the 8 pairs of a slot by the angles (c, s), or by minus them.  A register holds two neighbouring angles' values of one
+// vector, or, with neighbouring pairs, both values of a pair.
 template <bool INTERLEAVED, bool BACK>
-__device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float (&c)[8], const float (&s)[8]) {
+__device__ __forceinline__ void turn(f2 (&v)[8], const f2 (&c)[4], const f2 (&s)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float& a = INTERLEAVED ? (i < 4 ? lo[(2 * i) & 7] : hi[(2 * i) & 7]) : lo[i];
-    float& b = INTERLEAVED ? (i < 4 ? lo[(2 * i + 1) & 7] : hi[(2 * i + 1) & 7]) : hi[i];
-    const float sn = BACK ? -s[i] : s[i], x = a, z = b;
-    a = x * c[i] - z * sn;
-    b = z * c[i] + x * sn;
+  for (int i = 0; i < 4; ++i) {
+    float s0, s1;
+    unpair(s[i], s0, s1);
+    if constexpr (INTERLEAVED) {
+      float c0, c1;
+      unpair(c[i], c0, c1);
+      v[2 * i] = fma(swap(v[2 * i]), BACK ? pair(s0, -s0) : pair(-s0, s0), mul(v[2 * i], pair(c0, c0)));
+      v[2 * i + 1] = fma(swap(v[2 * i + 1]), BACK ? pair(s1, -s1) : pair(-s1, s1), mul(v[2 * i + 1], pair(c1, c1)));
+    } else {
+      const f2 n = pair(-s0, -s1), a = v[i], b = v[4 + i];
+      v[i] = fma(b, BACK ? s[i] : n, mul(a, c[i]));
+      v[4 + i] = fma(a, BACK ? n : s[i], mul(b, c[i]));
+    }
   }
 }
 
@@ -82,147 +107,171 @@ __device__ __forceinline__ float row_sum(float v) {
 
 // cos and sin of slot s at the token's position: (1, 0) behind the rotated part, NaN where the table does not have the
 // position, so that the mistake shows in the result.
-__device__ __forceinline__ void load_angles(const NormParams& p, int64_t b, int t, int s, float (&c)[8], float (&sn)[8]) {
+__device__ __forceinline__ void load_angles(const NormParams& p, int64_t b, int t, int s, bool on, f2 (&c)[4], f2 (&sn)[4]) {
   int64_t pos = t;
   if (p.pos) pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[b * p.pos_b + t] : reinterpret_cast<const int32_t*>(p.pos)[b * p.pos_b + t];
-  if (s * 16 < p.rot) {
-    if (pos >= 0 && pos < p.table) {
-      const float4* cp = reinterpret_cast<const float4*>(p.cos + pos * (p.rot / 2) + s * 8);
-      const float4* sp = reinterpret_cast<const float4*>(p.sin + pos * (p.rot / 2) + s * 8);
-      const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-      c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
-      sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w; sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = sn[i] = __uint_as_float(0x7fffffffu);
-    }
+  const bool turned = on && s * 16 < p.rot, there = pos >= 0 && pos < p.table;
+  if (turned && there) {
+    const ulonglong2* cp = reinterpret_cast<const ulonglong2*>(p.cos + pos * (p.rot / 2) + s * 8);
+    const ulonglong2* sp = reinterpret_cast<const ulonglong2*>(p.sin + pos * (p.rot / 2) + s * 8);
+    const ulonglong2 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+    c[0] = c0.x; c[1] = c0.y; c[2] = c1.x; c[3] = c1.y;
+    sn[0] = s0.x; sn[1] = s0.y; sn[2] = s1.x; sn[3] = s1.y;
   } else {
+    const float nan = __uint_as_float(0x7fffffffu);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { c[i] = 1.f; sn[i] = 0.f; }
+    for (int i = 0; i < 4; ++i) { c[i] = turned ? pair(nan, nan) : pair(1.f, 1.f); sn[i] = turned ? pair(nan, nan) : pair(0.f, 0.f); }
   }
 }
 
-// One warp = one token and `per_chunk` of its groups of 32 / LPR heads, q's heads before k's.
+// A warp's job: a token of q or of k and `per_chunk` of its groups of 32 / LPR heads.  All of q's jobs come before k's.
+struct NormJob { int64_t b; int t, g0, g1; };
+__device__ __forceinline__ NormJob norm_job(const NormParams& p, int which, int64_t job, int groups) {
+  NormJob j;
+  const int64_t token = job / p.chunks[which];
+  j.b = token / p.S;
+  j.t = (int)(token - j.b * p.S);
+  j.g0 = (int)(job - token * p.chunks[which]) * p.per_chunk[which];
+  j.g1 = min(j.g0 + p.per_chunk[which], groups);
+  return j;
+}
+
+// The next group's rows are on their way while a group is worked on.  Measured with 2 x 8192 tokens, 32 / 8 heads, d = 128,
+// bf16 (335 MB): see the figures at the end of this comment.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
-__global__ void __launch_bounds__(256) norm_rotary_fwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(256, 3) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
   const int lane = threadIdx.x & 31, s = lane % LPR, sub = lane / LPR;
   constexpr int HPG = 32 / LPR;
-  const int64_t job = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), token = job / p.chunks;
-  if (token >= (int64_t)p.B * p.S) return;
-  const int64_t b = token / p.S;
-  const int t = (int)(token - b * p.S), chunk = (int)(job - token * p.chunks);
   const bool on = s * 16 < p.d;
   int lo, hi;
   slot_offsets<INTERLEAVED>(s, p.rot, lo, hi);
-  float c[8], sn[8];
-  load_angles(p, b, t, on ? s : p.rot, c, sn);
-  const int groups[2] = {(p.H[0] + HPG - 1) / HPG, (p.H[1] + HPG - 1) / HPG};
-  const int g0 = chunk * p.per_chunk, g1 = min(g0 + p.per_chunk, groups[0] + groups[1]);
-  float wl[8], wh[8];
-  int have = -1;
-  for (int g = g0; g < g1; ++g) {
-    const int which = g >= groups[0], h = (which ? g - groups[0] : g) * HPG + sub;
-    if (which != have && on) { load_weight8<IS_BF16>(wl, p.w[which], p.w_f32, lo); load_weight8<IS_BF16>(wh, p.w[which], p.w_f32, hi); }
-    have = which;
-    const bool live = on && h < p.H[which];
-    float a[8] = {}, z[8] = {};
-    if (live) {
-      const uint16_t* x = p.x[which] + b * p.xs[which][0] + t * p.xs[which][1] + h * p.xs[which][2];
-      load8<IS_BF16>(a, x + lo);
-      load8<IS_BF16>(z, x + hi);
+  const int64_t tokens = (int64_t)p.B * p.S, q_jobs = tokens * p.chunks[0];
+  int64_t job = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int which = job >= q_jobs;
+  if (which) job -= q_jobs;
+  if (job >= tokens * p.chunks[which]) return;
+  const int H = p.H[which], groups = (H + HPG - 1) / HPG;
+  const NormJob j = norm_job(p, which, job, groups);
+  const int64_t xh = p.xs[which][2] * HPG, yh = p.ys[which][2] * HPG;
+  const uint16_t* x = p.x[which] + j.b * p.xs[which][0] + j.t * p.xs[which][1] + (int64_t)(j.g0 * HPG + sub) * p.xs[which][2];
+  uint16_t* y = p.y[which] + j.b * p.ys[which][0] + j.t * p.ys[which][1] + (int64_t)(j.g0 * HPG + sub) * p.ys[which][2];
+  auto load = [&](int g) {
+    Raw r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (on && g < j.g1 && g * HPG + sub < H) {
+      r.lo = __ldcs(reinterpret_cast<const uint4*>(x + lo));
+      r.hi = __ldcs(reinterpret_cast<const uint4*>(x + hi));
     }
-    float ss = 0.f;
+    x += xh;
+    return r;
+  };
+  Raw next = load(j.g0), after = load(j.g0 + 1);
+  f2 c[4], sn[4], w[8];
+  load_angles(p, j.b, j.t, s, on, c, sn);
+  if (on) load_weight<IS_BF16>(w, p.w[which], p.w_f32, lo, hi);
+#pragma unroll 1
+  for (int g = j.g0; g < j.g1; ++g) {
+    f2 v[8];
+    widen<IS_BF16>(v, next);
+    next = after;
+    after = load(g + 2);
+    f2 ss = mul(v[0], v[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + z[i] * z[i];
-    const float r = 1.f / sqrtf(row_sum<LPR>(ss) / p.d + p.eps);
-    if (!live) continue;
+    for (int i = 1; i < 8; ++i) ss = fma(v[i], v[i], ss);
+    const float r = 1.f / sqrtf(row_sum<LPR>(sum(ss)) * p.inv_d + p.eps);
     // (x w is exact where both have 8 bits, and r comes last: three roundings and r's)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { a[i] *= wl[i]; z[i] *= wh[i]; }
-    turn<INTERLEAVED, false>(a, z, c, sn);
+    for (int i = 0; i < 8; ++i) v[i] = mul(v[i], w[i]);
+    turn<INTERLEAVED, false>(v, c, sn);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { a[i] *= r; z[i] *= r; }
-    uint16_t* y = p.y[which] + b * p.ys[which][0] + t * p.ys[which][1] + h * p.ys[which][2];
-    store8<IS_BF16>(y + lo, a);
-    store8<IS_BF16>(y + hi, z);
+    for (int i = 0; i < 8; ++i) v[i] = mul(v[i], pair(r, r));
+    if (on && g * HPG + sub < H) store<IS_BF16>(y, lo, hi, v);
+    y += yh;
   }
 }
 
-// Warps walk the (token, chunk) jobs with a stride of the grid and keep the sums of dw of their slots in registers.
+// Warps walk q's jobs and then k's with a stride of the grid and keep the sums of dw of their slots in registers.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
-__global__ void __launch_bounds__(256) norm_rotary_bwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ float sums[];                                // [8 warps][2][LPR * 16]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane % LPR, sub = lane / LPR;
   constexpr int HPG = 32 / LPR;
   const bool on = s * 16 < p.d;
   int lo, hi;
   slot_offsets<INTERLEAVED>(s, p.rot, lo, hi);
-  const int groups[2] = {(p.H[0] + HPG - 1) / HPG, (p.H[1] + HPG - 1) / HPG};
-  float dw[2][16] = {};
-  const int64_t jobs = (int64_t)p.B * p.S * p.chunks;
-  for (int64_t job = (int64_t)blockIdx.x * 8 + warp; job < jobs; job += (int64_t)gridDim.x * 8) {
-    const int64_t token = job / p.chunks, b = token / p.S;
-    const int t = (int)(token - b * p.S), chunk = (int)(job - token * p.chunks);
-    float c[8], sn[8];
-    load_angles(p, b, t, on ? s : p.rot, c, sn);
-    const int g0 = chunk * p.per_chunk, g1 = min(g0 + p.per_chunk, groups[0] + groups[1]);
+  grid_dep_trigger();                                            // (the sum over the CTAs waits for this kernel's end)
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    f2 dw[8], w[8];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int from = which ? max(g0 - groups[0], 0) : g0, to = which ? g1 - groups[0] : min(g1, groups[0]);
-      if (from >= to) continue;
-      float wl[8], wh[8];
-      if (on) { load_weight8<IS_BF16>(wl, p.w[which], p.w_f32, lo); load_weight8<IS_BF16>(wh, p.w[which], p.w_f32, hi); }
-      for (int g = from; g < to; ++g) {
-        const int h = g * HPG + sub;
-        const bool live = on && h < p.H[which];
-        float a[8] = {}, z[8] = {}, ga[8] = {}, gz[8] = {};
+    for (int i = 0; i < 8; ++i) dw[i] = 0;
+    if (on) load_weight<IS_BF16>(w, p.w[which], p.w_f32, lo, hi);
+    const int H = p.H[which], groups = (H + HPG - 1) / HPG;
+    const int64_t jobs = (int64_t)p.B * p.S * p.chunks[which], xh = p.xs[which][2] * HPG, yh = p.ys[which][2] * HPG, dh = p.dys[which][2] * HPG;
+#pragma unroll 1
+    for (int64_t job = (int64_t)blockIdx.x * 8 + warp; job < jobs; job += (int64_t)gridDim.x * 8) {
+      const NormJob j = norm_job(p, which, job, groups);
+      const int h0 = j.g0 * HPG + sub;
+      const uint16_t* x = p.x[which] + j.b * p.xs[which][0] + j.t * p.xs[which][1] + h0 * p.xs[which][2];
+      const uint16_t* dy = p.dy[which] + j.b * p.dys[which][0] + j.t * p.dys[which][1] + h0 * p.dys[which][2];
+      uint16_t* y = p.y[which] + j.b * p.ys[which][0] + j.t * p.ys[which][1] + h0 * p.ys[which][2];
+      Raw nx, ng;
+      auto load = [&](int g) {
+        nx.lo = nx.hi = ng.lo = ng.hi = make_uint4(0, 0, 0, 0);
+        if (on && g < j.g1 && g * HPG + sub < H) {
+          nx.lo = __ldcs(reinterpret_cast<const uint4*>(x + lo));
+          nx.hi = __ldcs(reinterpret_cast<const uint4*>(x + hi));
+          ng.lo = __ldcs(reinterpret_cast<const uint4*>(dy + lo));
+          ng.hi = __ldcs(reinterpret_cast<const uint4*>(dy + hi));
+        }
+        x += xh;
+        dy += dh;
+      };
+      load(j.g0);
+      f2 c[4], sn[4];
+      load_angles(p, j.b, j.t, s, on, c, sn);
+#pragma unroll 1
+      for (int g = j.g0; g < j.g1; ++g) {
+        f2 v[8], d[8];
+        widen<IS_BF16>(v, nx);
+        widen<IS_BF16>(d, ng);
+        load(g + 1);
+        const bool live = on && g * HPG + sub < H;
+        turn<INTERLEAVED, true>(d, c, sn);
+        f2 ss = mul(v[0], v[0]), dot = mul(mul(d[0], w[0]), v[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) { ss = fma(v[i], v[i], ss); dot = fma(mul(d[i], w[i]), v[i], dot); }
+        const float r = 1.f / sqrtf(row_sum<LPR>(sum(ss)) * p.inv_d + p.eps), m = row_sum<LPR>(live ? sum(dot) : 0.f) * r * p.inv_d;
         if (live) {
-          const uint16_t* x = p.x[which] + b * p.xs[which][0] + t * p.xs[which][1] + h * p.xs[which][2];
-          const uint16_t* dy = p.dy[which] + b * p.dys[which][0] + t * p.dys[which][1] + h * p.dys[which][2];
-          load8<IS_BF16>(a, x + lo);
-          load8<IS_BF16>(z, x + hi);
-          load8<IS_BF16>(ga, dy + lo);
-          load8<IS_BF16>(gz, dy + hi);
-          turn<INTERLEAVED, true>(ga, gz, c, sn);
-        }
-        float ss = 0.f, dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss += a[i] * a[i] + z[i] * z[i];
-          dot += live ? ga[i] * wl[i] * a[i] + gz[i] * wh[i] * z[i] : 0.f;
+          for (int i = 0; i < 8; ++i) {
+            const f2 xr = mul(v[i], pair(r, r));
+            dw[i] = fma(d[i], xr, dw[i]);
+            v[i] = mul(fma(xr, pair(-m, -m), mul(d[i], w[i])), pair(r, r));
+          }
+          store<IS_BF16>(y, lo, hi, v);
         }
-        ss = row_sum<LPR>(ss);
-        dot = row_sum<LPR>(dot);
-        const float r = 1.f / sqrtf(ss / p.d + p.eps), m = dot * r * r / p.d;
-        if (!live) continue;
+        y += yh;
+      }
+    }
+    // the warp's rows side by side; the warps below, in a fixed order
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dw[which][i] += ga[i] * a[i] * r;
-          dw[which][8 + i] += gz[i] * z[i] * r;
-          a[i] = r * (ga[i] * wl[i] - a[i] * m);
-          z[i] = r * (gz[i] * wh[i] - z[i] * m);
-        }
-        uint16_t* y = p.y[which] + b * p.ys[which][0] + t * p.ys[which][1] + h * p.ys[which][2];
-        store8<IS_BF16>(y + lo, a);
-        store8<IS_BF16>(y + hi, z);
+    for (int i = 0; i < 8; ++i) {
+      float a[2];
+      unpair(dw[i], a[0], a[1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 16; o >= LPR; o >>= 1) a[e] += __shfl_xor_sync(0xffffffffu, a[e], o);
+        if (sub == 0 && on) sums[(warp * 2 + which) * LPR * 16 + (i < 4 ? lo + 2 * i : hi + 2 * i - 8) + e] = a[e];
       }
     }
   }
   if (!p.part) return;
-  // sub-rows of the warp, then the warps, in a fixed order
-#pragma unroll
-  for (int which = 0; which < 2; ++which)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = dw[which][i];
-#pragma unroll
-      for (int o = 16; o >= LPR; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (sub == 0 && on) sums[(warp * 2 + which) * LPR * 16 + (i < 8 ? lo + i : hi + i - 8)] = v;
-    }
   __syncthreads();
   for (int j = threadIdx.x; j < 2 * p.d; j += 256) {
     const int which = j >= p.d, at = which ? j - p.d : j;
     float v = 0.f;
+#pragma unroll
     for (int k = 0; k < 8; ++k) v += sums[(k * 2 + which) * LPR * 16 + at];
     p.part[(size_t)blockIdx.x * 2 * p.d + j] = v;
   }
@@ -260,12 +309,14 @@ int sm_count();
 static void norm_plan(const fm_norm_rotary_args* a, NormParams* p) {
   p->B = a->B; p->S = a->S; p->d = a->d;
   const int lpr = a->d <= 128 ? 8 : (a->d <= 256 ? 16 : 32), hpg = 32 / lpr;
-  const int groups = (a->Hq + hpg - 1) / hpg + (a->Hk + hpg - 1) / hpg;
   const int64_t tokens = (int64_t)a->B * a->S, warps = (int64_t)sm_count() * 64;
   const int64_t want = tokens > 0 ? (warps + tokens - 1) / tokens : 1;
-  p->chunks = (int)std::max<int64_t>(1, std::min<int64_t>(want, groups));
-  p->per_chunk = (groups + p->chunks - 1) / p->chunks;
-  if (p->per_chunk > 0) p->chunks = (groups + p->per_chunk - 1) / p->per_chunk;
+  for (int i = 0; i < 2; ++i) {
+    const int groups = ((i ? a->Hk : a->Hq) + hpg - 1) / hpg;
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(want, groups));
+    p->per_chunk[i] = (int)std::max<int64_t>(1, (groups + chunks - 1) / chunks);
+    p->chunks[i] = (groups + p->per_chunk[i] - 1) / p->per_chunk[i];
+  }
 }
 
 static int norm_params(const fm_norm_rotary_args* a, bool back, NormParams* p) {
@@ -301,13 +352,14 @@ static int norm_params(const fm_norm_rotary_args* a, bool back, NormParams* p) {
   p->cos = a->cos; p->sin = a->sin; p->pos = a->positions; p->pos64 = a->positions_64; p->pos_b = a->positions_stride;
   p->rot = a->rot; p->table = a->table; p->w_f32 = a->weight_f32;
   p->eps = a->eps;
+  p->inv_d = 1.f / (float)(a->d > 0 ? a->d : 1);
   p->part = nullptr;
   norm_plan(a, p);
   return FM_OK;
 }
 
 static int64_t norm_bwd_grid(const NormParams& p) {
-  const int64_t jobs = (int64_t)p.B * p.S * p.chunks, most = (int64_t)sm_count() * 2;
+  const int64_t jobs = (int64_t)p.B * p.S * std::max(p.chunks[0], p.chunks[1]), most = (int64_t)sm_count() * 2;
   const int64_t need = (jobs + 7) / 8;
   return need < 1 ? 1 : (need < most ? need : most);
 }
@@ -342,8 +394,8 @@ extern "C" FM_API int fm_norm_rotary_fwd(const fm_norm_rotary_args* a, void* str
   NormParams p;
   const int rc = norm_params(a, false, &p);
   if (rc) return rc;
-  const int64_t jobs = (int64_t)p.B * p.S * p.chunks;
-  if (jobs == 0 || p.per_chunk == 0) return FM_OK;
+  const int64_t jobs = (int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]);
+  if (jobs == 0) return FM_OK;
   return norm_dispatch(p, a, false, (jobs + 7) / 8, (cudaStream_t)stream);
 }
 
@@ -364,7 +416,7 @@ extern "C" FM_API int fm_norm_rotary_bwd(const fm_norm_rotary_args* a, void* str
     FM_REQUIRE(a->workspace && a->workspace_bytes >= (size_t)grid * 2 * p.d * sizeof(float) && ((uintptr_t)a->workspace & 15) == 0,
                FM_ERR_WORKSPACE, "fm_norm_rotary_bwd: workspace of %zu bytes", a->workspace_bytes);
     p.part = (float*)a->workspace;
-  } else if ((int64_t)p.B * p.S * p.per_chunk == 0) {
+  } else if ((int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]) == 0) {
     return FM_OK;
   }
   if (const int e = norm_dispatch(p, a, true, grid, (cudaStream_t)stream)) return e;
