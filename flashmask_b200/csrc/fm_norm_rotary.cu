@@ -136,8 +136,8 @@ __device__ __forceinline__ NormJob norm_job(const NormParams& p, int which, int6
   return j;
 }
 
-// The next group's rows are on their way while a group is worked on.  Measured with 2 x 8192 tokens, 32 / 8 heads, d = 128,
-// bf16 (335 MB): see the figures at the end of this comment.
+// Forward.  A warp has one job, and the rows of the next two groups are on their way while one is worked on: 2 x 8192 tokens,
+// 32 / 8 heads, d = 128, bf16 (335 MB) in 62 us, 5.4 TB/s; with the backward's stream through shared memory 70 us.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
 __global__ void __launch_bounds__(256, 3) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
   const int lane = threadIdx.x & 31, s = lane % LPR, sub = lane / LPR;
@@ -189,53 +189,153 @@ __global__ void __launch_bounds__(256, 3) norm_rotary_fwd_kernel(const __grid_co
   }
 }
 
-// Warps walk q's jobs and then k's with a stride of the grid and keep the sums of dw of their slots in registers.
+// A warp's stream of groups of rows: jobs `first`, `first` + `step`, .. of q or of k, a job being a token and some of its groups of
+// HPG = 32 / LPR heads.  Rows of x and dy are copied to shared memory DEPTH groups ahead, across jobs: a
+// lane copies what it will read itself, so nothing has to be waited for but the copies; and the angles of a job's token go to a ring
+// of their own, copied by one row's lanes for all.  (A group read in this step, DEPTH ahead of it, and the angles of the job behind:
+// DEPTH + 2 entries where every job is one group.)
+constexpr int NORM_DEPTH = 4;
+template <int LPR>
+struct NormStream {
+  static constexpr int HPG = 32 / LPR;
+  static constexpr int STAGE = 4 * 512, ANGLES = LPR * 64, BYTES = NORM_DEPTH * STAGE + (NORM_DEPTH + 2) * ANGLES;    // of a warp
+  const NormParams& p;
+  const int which, lane, s, sub, lo, hi, H, groups;
+  const bool on;
+  const uint32_t ring, angles;
+  const int jobs, step;
+  // the copies' side
+  int job, next_pos, g, g1, stage, entry;
+  const uint16_t *x, *dy;
+
+  __device__ __forceinline__ NormStream(const NormParams& p_, int which_, uint32_t smem, int first, int step_, int lo_, int hi_)
+      : p(p_), which(which_), lane(threadIdx.x & 31), s(lane % LPR), sub(lane / LPR), lo(lo_), hi(hi_), H(p_.H[which_]),
+        groups((p_.H[which_] + HPG - 1) / HPG), on(s * 16 < p_.d), ring(smem), angles(smem + NORM_DEPTH * STAGE),
+        jobs(p_.B * p_.S * p_.chunks[which_]), step(step_), job(first), g(0), g1(0), stage(0), entry(0) {
+    next_pos = position(job);
+    begin();
+  }
+  __device__ __forceinline__ void place(int j, int64_t& b, int& t, int& g0, int& g1_) const {
+    const int token = p.chunks[which] == 1 ? j : j / p.chunks[which], seq = token / p.S;
+    b = seq;
+    t = token - seq * p.S;
+    g0 = (j - token * p.chunks[which]) * p.per_chunk[which];
+    g1_ = min(g0 + p.per_chunk[which], groups);
+  }
+  // the position of job j's token, or -1: not in the tables
+  __device__ __forceinline__ int position(int j) const {
+    if (j >= jobs) return 0;
+    int64_t b; int t, g0, e;
+    place(j, b, t, g0, e);
+    if (!p.pos) return t;
+    const int64_t pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[b * p.pos_b + t] : reinterpret_cast<const int32_t*>(p.pos)[b * p.pos_b + t];
+    return pos >= 0 && pos < p.table ? (int)pos : -1;
+  }
+  // The job's rows from its first group on, and its angles: NaN where the tables do not have the position, so that the
+  // mistake shows in the result.
+  __device__ __forceinline__ void begin() {
+    if (job >= jobs) return;
+    int64_t b; int t, g0;
+    place(job, b, t, g0, g1);
+    g = g0;
+    const int h = g0 * HPG + sub;
+    x = p.x[which] + b * p.xs[which][0] + t * p.xs[which][1] + h * p.xs[which][2];
+    dy = p.dy[which] + b * p.dys[which][0] + t * p.dys[which][1] + h * p.dys[which][2];
+    const int pos = next_pos;
+    next_pos = position(job + step);
+    if (sub == 0) {
+      const uint32_t to = angles + entry * ANGLES + s * 16;
+      const bool turned = s * 16 < p.rot;
+      if (turned && pos >= 0) {
+        const float *c = p.cos + (int64_t)pos * (p.rot / 2) + s * 8, *n = p.sin + (int64_t)pos * (p.rot / 2) + s * 8;
+        cp_async16(to, c, true);
+        cp_async16(to + LPR * 16, c + 4, true);
+        cp_async16(to + LPR * 32, n, true);
+        cp_async16(to + LPR * 48, n + 4, true);
+      } else {                                                   // (cos, sin) = (1, 0) behind the rotated part
+        const uint32_t c = turned ? 0x7fffffffu : 0x3f800000u, n = turned ? 0x7fffffffu : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(to + LPR * 16 * i), "r"(i < 2 ? c : n) : "memory");
+      }
+    }
+    entry = entry == NORM_DEPTH + 1 ? 0 : entry + 1;
+  }
+  // The copies of the next group; one commit for every call.
+  __device__ __forceinline__ void fetch() {
+    if (job < jobs) {
+      const bool live = on && g * HPG + sub < H;
+      const uint32_t to = ring + stage * STAGE + lane * 16;
+      cp_async16(to, live ? x + lo : p.x[which], live);
+      cp_async16(to + 512, live ? x + hi : p.x[which], live);
+      x += HPG * p.xs[which][2];
+      cp_async16(to + 1024, live ? dy + lo : p.dy[which], live);
+      cp_async16(to + 1536, live ? dy + hi : p.dy[which], live);
+      dy += HPG * p.dys[which][2];
+      if (++g == g1) { job += step; begin(); }
+    }
+    stage = stage + 1 == NORM_DEPTH ? 0 : stage + 1;
+    cp_async_commit();
+  }
+};
+
+__device__ __forceinline__ uint4 lds_vec(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+template <int LPR>
+__device__ __forceinline__ void read_angles(f2 (&c)[4], f2 (&sn)[4], uint32_t at) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 a = lds_vec(at + LPR * 16 * i), b = lds_vec(at + LPR * 16 * (2 + i));
+    c[2 * i] = pair(__uint_as_float(a.x), __uint_as_float(a.y)); c[2 * i + 1] = pair(__uint_as_float(a.z), __uint_as_float(a.w));
+    sn[2 * i] = pair(__uint_as_float(b.x), __uint_as_float(b.y)); sn[2 * i + 1] = pair(__uint_as_float(b.z), __uint_as_float(b.w));
+  }
+}
+
+// Backward.  Warps walk q's jobs and then k's with a stride of the grid and keep the sums of dw of their slots in registers.
+// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 90 us, 5.6 TB/s; with the next group's rows in registers 110 us.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
 __global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
-  extern __shared__ float sums[];                                // [8 warps][2][LPR * 16]
+  using Stream = NormStream<LPR>;
+  constexpr int HPG = Stream::HPG;
+  extern __shared__ __align__(128) unsigned char smem[];         // [8 warps] rings, sums [8][2][LPR * 16]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane % LPR, sub = lane / LPR;
-  constexpr int HPG = 32 / LPR;
   const bool on = s * 16 < p.d;
   int lo, hi;
   slot_offsets<INTERLEAVED>(s, p.rot, lo, hi);
+  float* sums = reinterpret_cast<float*>(smem + 8 * Stream::BYTES);
   grid_dep_trigger();                                            // (the sum over the CTAs waits for this kernel's end)
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
-    f2 dw[8], w[8];
+    const int step = gridDim.x * 8;
+    __syncwarp();
+    Stream in(p, which, smem_u32(smem) + warp * Stream::BYTES, blockIdx.x * 8 + warp, step, lo, hi);
+#pragma unroll 1
+    for (int i = 0; i < NORM_DEPTH; ++i) in.fetch();
+    f2 w[8], dw[8];
+    if (on) load_weight<IS_BF16>(w, p.w[which], p.w_f32, lo, hi);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[i] = 0;
-    if (on) load_weight<IS_BF16>(w, p.w[which], p.w_f32, lo, hi);
-    const int H = p.H[which], groups = (H + HPG - 1) / HPG;
-    const int64_t jobs = (int64_t)p.B * p.S * p.chunks[which], xh = p.xs[which][2] * HPG, yh = p.ys[which][2] * HPG, dh = p.dys[which][2] * HPG;
+    int stage = 0, entry = 0;
+    const int64_t yh = p.ys[which][2] * HPG;
 #pragma unroll 1
-    for (int64_t job = (int64_t)blockIdx.x * 8 + warp; job < jobs; job += (int64_t)gridDim.x * 8) {
-      const NormJob j = norm_job(p, which, job, groups);
-      const int h0 = j.g0 * HPG + sub;
-      const uint16_t* x = p.x[which] + j.b * p.xs[which][0] + j.t * p.xs[which][1] + h0 * p.xs[which][2];
-      const uint16_t* dy = p.dy[which] + j.b * p.dys[which][0] + j.t * p.dys[which][1] + h0 * p.dys[which][2];
-      uint16_t* y = p.y[which] + j.b * p.ys[which][0] + j.t * p.ys[which][1] + h0 * p.ys[which][2];
-      Raw nx, ng;
-      auto load = [&](int g) {
-        nx.lo = nx.hi = ng.lo = ng.hi = make_uint4(0, 0, 0, 0);
-        if (on && g < j.g1 && g * HPG + sub < H) {
-          nx.lo = __ldcs(reinterpret_cast<const uint4*>(x + lo));
-          nx.hi = __ldcs(reinterpret_cast<const uint4*>(x + hi));
-          ng.lo = __ldcs(reinterpret_cast<const uint4*>(dy + lo));
-          ng.hi = __ldcs(reinterpret_cast<const uint4*>(dy + hi));
-        }
-        x += xh;
-        dy += dh;
-      };
-      load(j.g0);
-      f2 c[4], sn[4];
-      load_angles(p, j.b, j.t, s, on, c, sn);
+    for (int job = blockIdx.x * 8 + warp; job < in.jobs; job += step) {
+      int64_t b; int t, g, g1;
+      in.place(job, b, t, g, g1);
+      uint16_t* y = p.y[which] + b * p.ys[which][0] + t * p.ys[which][1] + (int64_t)(g * HPG + sub) * p.ys[which][2];
 #pragma unroll 1
-      for (int g = j.g0; g < j.g1; ++g) {
-        f2 v[8], d[8];
-        widen<IS_BF16>(v, nx);
-        widen<IS_BF16>(d, ng);
-        load(g + 1);
-        const bool live = on && g * HPG + sub < H;
+      for (; g < g1; ++g) {
+        cp_async_wait<NORM_DEPTH - 1>();
+        __syncwarp();                                            // the angles were copied by other lanes
+        const uint32_t from = in.ring + stage * Stream::STAGE + lane * 16;
+        stage = stage + 1 == NORM_DEPTH ? 0 : stage + 1;
+        f2 v[8], d[8], c[4], sn[4];
+        widen<IS_BF16>(v, Raw{lds_vec(from), lds_vec(from + 512)});
+        widen<IS_BF16>(d, Raw{lds_vec(from + 1024), lds_vec(from + 1536)});
+        read_angles<LPR>(c, sn, in.angles + entry * Stream::ANGLES + s * 16);
+        in.fetch();
+        const bool live = on && g * HPG + sub < in.H;
         turn<INTERLEAVED, true>(d, c, sn);
         f2 ss = mul(v[0], v[0]), dot = mul(mul(d[0], w[0]), v[0]);
 #pragma unroll
@@ -252,7 +352,9 @@ __global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_co
         }
         y += yh;
       }
+      entry = entry == NORM_DEPTH + 1 ? 0 : entry + 1;
     }
+    cp_async_wait<0>();
     // the warp's rows side by side; the warps below, in a fixed order
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -355,35 +457,37 @@ static int norm_params(const fm_norm_rotary_args* a, bool back, NormParams* p) {
   p->inv_d = 1.f / (float)(a->d > 0 ? a->d : 1);
   p->part = nullptr;
   norm_plan(a, p);
+  FM_REQUIRE((int64_t)a->B * a->S * std::max(p->chunks[0], p->chunks[1]) < INT_MAX / 2, FM_ERR_UNSUPPORTED, "norm_rotary: too many tokens for one call");
   return FM_OK;
 }
 
+// Two CTAs of the backward per SM, as its registers allow.
 static int64_t norm_bwd_grid(const NormParams& p) {
   const int64_t jobs = (int64_t)p.B * p.S * std::max(p.chunks[0], p.chunks[1]), most = (int64_t)sm_count() * 2;
-  const int64_t need = (jobs + 7) / 8;
-  return need < 1 ? 1 : (need < most ? need : most);
+  return std::max<int64_t>(1, std::min((jobs + 7) / 8, most));
 }
 
-template <bool IS_BF16, bool IL>
-static int norm_launch(const NormParams& p, bool back, int64_t grid, cudaStream_t s) {
-#define FM_NORM(LPR)                                                                                         \
-  do {                                                                                                       \
-    if (back) norm_rotary_bwd_kernel<IS_BF16, IL, LPR><<<(unsigned)grid, 256, 8 * 2 * LPR * 16 * sizeof(float), s>>>(p); \
-    else norm_rotary_fwd_kernel<IS_BF16, IL, LPR><<<(unsigned)grid, 256, 0, s>>>(p);                         \
-  } while (0)
-  if (p.d <= 128) FM_NORM(8);
-  else if (p.d <= 256) FM_NORM(16);
-  else FM_NORM(32);
-#undef FM_NORM
+template <bool IS_BF16, bool IL, int LPR>
+static int norm_launch(const NormParams& p, bool back, cudaStream_t s) {
+  if (back) {
+    auto kern = norm_rotary_bwd_kernel<IS_BF16, IL, LPR>;
+    constexpr int smem = 8 * NormStream<LPR>::BYTES + 8 * 2 * LPR * 16 * 4;
+    FM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kern<<<(unsigned)norm_bwd_grid(p), 256, smem, s>>>(p);
+  } else {
+    const int64_t jobs = (int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]);
+    norm_rotary_fwd_kernel<IS_BF16, IL, LPR><<<(unsigned)((jobs + 7) / 8), 256, 0, s>>>(p);
+  }
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   return FM_OK;
 }
 
-static int norm_dispatch(const NormParams& p, const fm_norm_rotary_args* a, bool back, int64_t grid, cudaStream_t s) {
-  FM_REQUIRE(grid <= INT_MAX, FM_ERR_UNSUPPORTED, "norm_rotary: too many tokens for one call");
-  if (a->dtype == FM_DTYPE_BF16) return a->interleaved ? norm_launch<true, true>(p, back, grid, s) : norm_launch<true, false>(p, back, grid, s);
-  return a->interleaved ? norm_launch<false, true>(p, back, grid, s) : norm_launch<false, false>(p, back, grid, s);
+static int norm_dispatch(const NormParams& p, const fm_norm_rotary_args* a, bool back, cudaStream_t s) {
+#define FM_NORM(BF, IL) (p.d <= 128 ? norm_launch<BF, IL, 8>(p, back, s) : p.d <= 256 ? norm_launch<BF, IL, 16>(p, back, s) : norm_launch<BF, IL, 32>(p, back, s))
+  if (a->dtype == FM_DTYPE_BF16) return a->interleaved ? FM_NORM(true, true) : FM_NORM(true, false);
+  return a->interleaved ? FM_NORM(false, true) : FM_NORM(false, false);
+#undef FM_NORM
 }
 
 }  // namespace fm
@@ -396,7 +500,7 @@ extern "C" FM_API int fm_norm_rotary_fwd(const fm_norm_rotary_args* a, void* str
   if (rc) return rc;
   const int64_t jobs = (int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]);
   if (jobs == 0) return FM_OK;
-  return norm_dispatch(p, a, false, (jobs + 7) / 8, (cudaStream_t)stream);
+  return norm_dispatch(p, a, false, (cudaStream_t)stream);
 }
 
 extern "C" FM_API size_t fm_norm_rotary_bwd_workspace_bytes(const fm_norm_rotary_args* a) {
@@ -419,7 +523,7 @@ extern "C" FM_API int fm_norm_rotary_bwd(const fm_norm_rotary_args* a, void* str
   } else if ((int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]) == 0) {
     return FM_OK;
   }
-  if (const int e = norm_dispatch(p, a, true, grid, (cudaStream_t)stream)) return e;
+  if (const int e = norm_dispatch(p, a, true, (cudaStream_t)stream)) return e;
   if (!sums) return FM_OK;
   const NormSumParams q{p.part, (int)grid, p.d, a->weight_f32, a->dtype == FM_DTYPE_BF16, {a->dq_weight, a->dk_weight}};
   FM_CUDA_TRY(launch_dependent(norm_rotary_dw_kernel, dim3((unsigned)((2 * p.d + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, q));
