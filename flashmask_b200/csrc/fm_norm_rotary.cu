@@ -411,7 +411,7 @@ int sm_count();
 static void norm_plan(const fm_norm_rotary_args* a, NormParams* p) {
   p->B = a->B; p->S = a->S; p->d = a->d;
   const int lpr = a->d <= 128 ? 8 : (a->d <= 256 ? 16 : 32), hpg = 32 / lpr;
-  const int64_t tokens = (int64_t)a->B * a->S, warps = (int64_t)sm_count() * 64;
+  const int64_t tokens = (int64_t)a->B * a->S, warps = (int64_t)sm_count() * 24;
   const int64_t want = tokens > 0 ? (warps + tokens - 1) / tokens : 1;
   for (int i = 0; i < 2; ++i) {
     const int groups = ((i ? a->Hk : a->Hq) + hpg - 1) / hpg;
