@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <climits>
 #include <cstdio>
 
@@ -47,6 +48,18 @@ cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, dim3 block, size_t s
   cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = s;
   cfg.attrs = &attr; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
+// Allows `kern` that much dynamic shared memory on the current device; asked for once per kernel and device.
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  const cudaError_t r = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (r == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return r;
 }
 
 #define FM_REQUIRE(cond, code, ...)     \

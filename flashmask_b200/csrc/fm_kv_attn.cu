@@ -700,7 +700,8 @@ static int launch_kv_attn(const KvAttnParams& p, cudaStream_t s) {
   using Cfg = KvCfg<DK, VC, NT>;
   auto kern = kv_attn_kernel<DK, VC, NT, INT8, FULL>;
   const size_t smem = Cfg::FIXED + (size_t)(p.B + 1) * 4;
-  FM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::FIXED + (KV_MAX_B + 1) * 4));
+  static std::atomic<uint64_t> done{0};
+  FM_CUDA_TRY(allow_smem(kern, Cfg::FIXED + (KV_MAX_B + 1) * 4, done));
   kern<<<p.n_cta, KV_WARPS * 32, smem, s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());

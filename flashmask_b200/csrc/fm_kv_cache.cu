@@ -15,6 +15,13 @@ struct KvWriteParams {
   int B, S;
 };
 
+// The part of 256 threads that walks rows of `upr` units of 8 values: thread = unit `col` of rows row0, row0 + step, ..
+struct RowWalk { int row0, step, col; };
+__device__ __forceinline__ RowWalk row_walk(int upr) {
+  const int step = 256 / upr, row0 = threadIdx.x / upr;
+  return {row0 < step ? row0 : INT_MAX / 2, step, (int)threadIdx.x - row0 * upr};
+}
+
 // One CTA = one page of one kv head, K or V (blockIdx.y = 2 * head + which), of the pages that the new tokens of sequence
 // blockIdx.z reach.  It reads its tokens once, keeps them in registers while the CTA finds the largest magnitude, and
 // writes one byte for every two that it read.  Bound by HBM: 3 bytes a value.
@@ -22,9 +29,8 @@ struct KvWriteParams {
 // of the earlier tokens is rounded on the new grid.  Slots behind the last new token are left as they are.
 // VEC = units of 8 values that a thread holds.
 template <bool IS_BF16, bool INT8, int VEC>
-__global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteParams p) {
-  __shared__ float s_max[8];
-  __shared__ int s_nan[8];
+__global__ void __launch_bounds__(256, VEC <= 4 ? 5 : (VEC <= 8 ? 2 : 1)) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
+  __shared__ uint32_t s_max[8];
   const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, P = 1 << p.g.page_log2;
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int start = p.start[b];
@@ -35,83 +41,88 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteParams p) {
   if (base > last || base < 0) return;
   const int page = kv_page(p.g, p.table + b * p.g.table_stride, base);
   if (page < 0) return;
-  const int w = p.width[which], upr = w >> 3;                     // units of 8 values in a row
+  const int w = p.width[which];
+  const RowWalk at = row_walk(w >> 3);
   const int lo = max(first - base, 0), hi = min(last - base + 1, P);       // slots [lo, hi) are new
-  uint8_t* pay = p.pay[which] + ((size_t)page * p.g.Hkv + h) * P * w;
+  uint8_t* pay = p.pay[which] + ((size_t)page * p.g.Hkv + h) * P * w + at.col * 8;
   float* scale = p.scale[which] + (size_t)page * p.g.Hkv + h;
-  const uint16_t* src = p.src[which] + b * p.stride[which][0] + h * p.stride[which][2];
   const int64_t ss = p.stride[which][1];
+  const uint16_t* src = p.src[which] + b * p.stride[which][0] + h * p.stride[which][2] + (base - start) * ss + at.col * 8;
   const float old = lo > 0 ? *scale : 0.f;
-  const int n_units = (hi - lo) * upr;
   uint4 x[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const int u = threadIdx.x + i * blockDim.x;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (u < n_units) {
-      const int row = u / upr;
-      x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)(base + lo + row - start) * ss + (u - row * upr) * 8));
-    }
+    const int row = lo + at.row0 + i * at.step;
+    x[i] = row < hi ? __ldcs(reinterpret_cast<const uint4*>(src + row * ss)) : make_uint4(0, 0, 0, 0);
   }
-  float amax = 0.f;
-  bool bad = false;
+  // the largest magnitude, as bits: of 16-bit floats these have the order of the values, infinities and NaN on top
+  constexpr uint32_t INF = IS_BF16 ? 0x7f80u : 0x7c00u;
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float2 f = unpack2<IS_BF16>(v[c]);
-      const float a = fabsf(f.x), d = fabsf(f.y);
-      // (a value that is no number does not set the scale)
-      if (a <= 3.4e38f) amax = fmaxf(amax, a); else bad = true;
-      if (d <= 3.4e38f) amax = fmaxf(amax, d); else bad = true;
-    }
+    top = __vmaxu2(top, __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu), __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu)));
   }
+  top = max(top & 0xffffu, top >> 16);
+  const int warp = threadIdx.x >> 5;
+  auto largest = [&](uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) s_max[warp] = v;
+    __syncthreads();
 #pragma unroll
-  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  bad = __any_sync(0xffffffffu, bad);
-  const int warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-  if ((threadIdx.x & 31) == 0) { s_max[warp] = amax; s_nan[warp] = bad; }
-  __syncthreads();
-  for (int i = 0; i < n_warps; ++i) { amax = fmaxf(amax, s_max[i]); bad |= s_nan[i] != 0; }
-  int e = cache_exponent<INT8>(amax);
+    for (int i = 0; i < 8; ++i) v = max(v, s_max[i]);
+    return v;
+  };
+  top = largest(top);
+  const bool bad = top >= INF;
+  if (bad) {
+    // What is no number does not set the scale and has no payload: NaN in e4m3, 0 in int8, where the scale says it.
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      uint32_t* v = reinterpret_cast<uint32_t*>(&x[i]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t l = v[c] & 0x7fffu, u = v[c] >> 16 & 0x7fffu;
+        if (l < INF) top = max(top, l); else v[c] = (v[c] & 0xffff0000u) | (INT8 ? 0u : 0x7fffu);
+        if (u < INF) top = max(top, u); else v[c] = (v[c] & 0xffffu) | (INT8 ? 0u : 0x7fff0000u);
+      }
+    }
+    __syncthreads();
+    top = largest(top);
+  }
+  int e = cache_exponent<INT8>(unpack2<IS_BF16>(top).x);
   const bool old_nan = INT8 && lo > 0 && !(old > 0.f);           // a NaN scale stays until the page is started again
   const int e_old = (int)(__float_as_uint(old) >> 23 & 0xff) - 127;
   if (lo > 0 && !old_nan) e = max(e, min(max(e_old, kCacheMinExp), kCacheMaxExp<INT8>));
   const float inv = exp2_int(-e);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const int u = threadIdx.x + i * blockDim.x;
-    if (u < n_units) {
-      const int row = u / upr;
+    const int row = lo + at.row0 + i * at.step;
+    if (row < hi) {
       const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
       uint32_t r[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        float2 f = unpack2<IS_BF16>(v[c]);
-        // what is no number has no payload: NaN in e4m3, 0 in int8, where the scale says it
-        const float none = INT8 ? 0.f : __uint_as_float(0x7fffffffu);
-        if (!(fabsf(f.x) <= 3.4e38f)) f.x = none;
-        if (!(fabsf(f.y) <= 3.4e38f)) f.y = none;
+        const float2 f = unpack2<IS_BF16>(v[c]);
         r[c] = to_payload2<INT8>(f.x * inv, f.y * inv);
       }
-      *reinterpret_cast<uint2*>(pay + (size_t)(lo + row) * w + (u - row * upr) * 8) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+      *reinterpret_cast<uint2*>(pay + row * w) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
     }
   }
   if (lo > 0 && !old_nan && e > e_old) {
     const float f = exp2_int(max(e_old - e, -126));
-    for (int u = threadIdx.x; u < lo * upr; u += blockDim.x) {
-      uint2* at = reinterpret_cast<uint2*>(pay) + u;
-      uint2 v = *at;
+    for (int row = at.row0; row < lo; row += at.step) {
+      uint2* to = reinterpret_cast<uint2*>(pay + row * w);
+      uint2 v = *to;
       float a[4];
       payload_f32<INT8>(v.x, a);
       v.x = to_payload2<INT8>(a[0] * f, a[1] * f) | to_payload2<INT8>(a[2] * f, a[3] * f) << 16;
       payload_f32<INT8>(v.y, a);
       v.y = to_payload2<INT8>(a[0] * f, a[1] * f) | to_payload2<INT8>(a[2] * f, a[3] * f) << 16;
-      *at = v;
+      *to = v;
     }
   }
-  // every thread has read the old scale (the barrier above), so it can go
+  // every thread has read the old scale (the barriers above), so it can go
   if (threadIdx.x == 0) *scale = INT8 && (bad || old_nan) ? __uint_as_float(0x7fffffffu) : exp2_int(e);
 }
 
@@ -124,53 +135,53 @@ struct KvReadParams {
   int B, S;
 };
 
-// dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  A thread takes 8 values at a time (8
-// bytes in, 16 out, neighbouring threads neighbouring units of the output) and has READ_ILP of them in flight, since each
-// is behind a page number and next to a scale.  Bound by HBM: 3 bytes a value.
+// dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  One CTA = the rows in one page of one kv
+// head, K or V, as in the write: the page and its scale are looked up once, and a thread has READ_ILP units of 8 bytes
+// in flight.  Bound by HBM: 3 bytes a value.
 constexpr int READ_ILP = 4;
 template <bool IS_BF16, bool INT8>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
-  const int b = blockIdx.y, which = blockIdx.z, w = p.width[which], upr = w >> 3, P = 1 << p.g.page_log2;
-  const uint32_t per_row = p.g.Hkv * upr;
-  const int64_t n_units = (int64_t)p.S * per_row;
-  const int start = p.start[b], len = kv_len(p.g, p.seqlens[b]);
-  const int32_t* row = p.table + b * p.g.table_stride;
-  uint16_t* dst = p.dst[which] + (size_t)b * p.S * p.g.Hkv * w;
-  const int64_t u0 = (int64_t)blockIdx.x * (256 * READ_ILP) + threadIdx.x;
-  uint2 v[READ_ILP];
-  float sc[READ_ILP];
-#pragma unroll
-  for (int i = 0; i < READ_ILP; ++i) {
-    const int64_t u = u0 + i * 256;
-    v[i] = make_uint2(0, 0);
-    sc[i] = 0.f;
-    if (u < n_units) {
-      const int s = (int)(u / per_row);
-      const uint32_t r = (uint32_t)(u - (int64_t)s * per_row), h = r / upr, c = r - h * upr;
-      const int64_t pos = (int64_t)start + s;
-      const int page = pos >= 0 && pos < len ? kv_page(p.g, row, (int)pos) : -1;
-      if (page >= 0) {
-        const size_t ph = (size_t)page * p.g.Hkv + h;
-        v[i] = __ldcs(reinterpret_cast<const uint2*>(p.pay[which] + (ph * P + (pos & (P - 1))) * w + c * 8));
-        sc[i] = __ldg(p.scale[which] + ph);
-      }
-    }
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadParams p) {
+  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, w = p.width[which], P = 1 << p.g.page_log2;
+  const int64_t start = p.start[b], base = ((start >> p.g.page_log2) + blockIdx.x) << p.g.page_log2;      // (rounds down below 0 too)
+  if (base >= start + p.S) return;
+  const int len = kv_len(p.g, p.seqlens[b]);
+  const int page = base >= 0 && base < len ? kv_page(p.g, p.table + b * p.g.table_stride, (int)base) : -1;
+  const int lo = base < start ? (int)(start - base) : 0, hi = (int)min((int64_t)P, start + p.S - base);    // slots that are asked for
+  const int valid = page >= 0 ? (int)min((int64_t)P, len - base) : 0;                                      // slots that hold tokens
+  const RowWalk at = row_walk(w >> 3);
+  const uint8_t* pay = p.pay[which];
+  float scale = 0.f;
+  if (page >= 0) {
+    const size_t ph = (size_t)page * p.g.Hkv + h;
+    pay += ph * P * w + at.col * 8;
+    scale = __ldg(p.scale[which] + ph);
   }
+  const int64_t out_row = (int64_t)p.g.Hkv * w;
+  uint16_t* dst = p.dst[which] + ((int64_t)b * p.S + (base - start)) * out_row + h * w + at.col * 8;
+  for (int row0 = lo + at.row0; row0 < hi; row0 += READ_ILP * at.step) {
+    uint2 v[READ_ILP];
 #pragma unroll
-  for (int i = 0; i < READ_ILP; ++i) {
-    const int64_t u = u0 + i * 256;
-    if (u >= n_units) break;
-    float a[4], c[4];
-    payload_f32<INT8>(v[i].x, a);
-    payload_f32<INT8>(v[i].y, c);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a[j] *= sc[i]; c[j] *= sc[i];
-      // the 8-bit grid reaches a little beyond fp16; NaN passes
-      if (!IS_BF16) { if (fabsf(a[j]) > 65504.f) a[j] = copysignf(65504.f, a[j]); if (fabsf(c[j]) > 65504.f) c[j] = copysignf(65504.f, c[j]); }
+    for (int i = 0; i < READ_ILP; ++i) {
+      const int row = row0 + i * at.step;
+      v[i] = row < hi && row < valid ? __ldcs(reinterpret_cast<const uint2*>(pay + row * w)) : make_uint2(0, 0);
     }
-    *reinterpret_cast<uint4*>(dst + u * 8) = make_uint4(pack2<IS_BF16>(a[0], a[1]), pack2<IS_BF16>(a[2], a[3]),
-                                                         pack2<IS_BF16>(c[0], c[1]), pack2<IS_BF16>(c[2], c[3]));
+#pragma unroll
+    for (int i = 0; i < READ_ILP; ++i) {
+      const int row = row0 + i * at.step;
+      if (row >= hi) break;
+      float a[4], c[4];
+      payload_f32<INT8>(v[i].x, a);
+      payload_f32<INT8>(v[i].y, c);
+      const float sc = row < valid ? scale : 0.f;                // (a NaN scale is no token's)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a[j] *= sc; c[j] *= sc;
+        // the 8-bit grid reaches a little beyond fp16; NaN passes
+        if (!IS_BF16) { if (fabsf(a[j]) > 65504.f) a[j] = copysignf(65504.f, a[j]); if (fabsf(c[j]) > 65504.f) c[j] = copysignf(65504.f, c[j]); }
+      }
+      *reinterpret_cast<uint4*>(dst + row * out_row) = make_uint4(pack2<IS_BF16>(a[0], a[1]), pack2<IS_BF16>(a[2], a[3]),
+                                                                  pack2<IS_BF16>(c[0], c[1]), pack2<IS_BF16>(c[2], c[3]));
+    }
   }
 }
 
@@ -235,14 +246,14 @@ int kv_geometry(const fm_kv_cache* c, const fm_kv_args* a, KvGeom* g) {
   return FM_OK;
 }
 
+// Pages that S tokens reach wherever the first falls.
+static unsigned pages_of(int S, int page_size) { return (unsigned)(((int64_t)S + page_size - 2) / page_size + 1); }
+
 template <bool IS_BF16, bool INT8>
 static int launch_write(const KvWriteParams& p, int page_size, int width_max, cudaStream_t s) {
-  const int units = page_size * width_max / 8;                     // <= 4096
-  const int threads = std::min(256, (units + 31) / 32 * 32);
-  const int64_t pages = ((int64_t)p.S + page_size - 2) / page_size + 1;      // wherever the first token falls
-  const dim3 grid((unsigned)pages, 2 * p.g.Hkv, p.B);
-  const int vec = (units + threads - 1) / threads;
-#define FM_KV_WRITE(N) if (vec <= N) { kv_write_kernel<IS_BF16, INT8, N><<<grid, threads, 0, s>>>(p); }
+  const int step = 256 / (width_max / 8), vec = (std::min(page_size, p.S) + step - 1) / step;      // <= 16
+  const dim3 grid(pages_of(p.S, page_size), 2 * p.g.Hkv, p.B);
+#define FM_KV_WRITE(N) if (vec <= N) { kv_write_kernel<IS_BF16, INT8, N><<<grid, 256, 0, s>>>(p); }
   FM_KV_WRITE(1) else FM_KV_WRITE(2) else FM_KV_WRITE(4) else FM_KV_WRITE(8) else FM_KV_WRITE(16)
 #undef FM_KV_WRITE
   count_launches(1);
@@ -296,9 +307,7 @@ extern "C" FM_API int fm_kv_read(const fm_kv_cache* c, const fm_kv_args* a, void
   p.width[0] = c->d; p.width[1] = c->dv;
   p.table = a->page_table; p.start = a->start; p.seqlens = a->seqlens;
   p.B = a->B; p.S = a->S;
-  const int64_t units = (int64_t)a->S * c->Hkv * ((c->d > c->dv ? c->d : c->dv) / 8), per = 256 * READ_ILP;
-  FM_REQUIRE((units + per - 1) / per <= INT_MAX, FM_ERR_UNSUPPORTED, "fm_kv_read: too many tokens for one call");
-  const dim3 grid((unsigned)((units + per - 1) / per), a->B, 2);
+  const dim3 grid(pages_of(a->S, c->page_size), 2 * c->Hkv, a->B);
   const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
   cudaStream_t s = (cudaStream_t)stream;
   if (bf) { if (i8) kv_read_kernel<true, true><<<grid, 256, 0, s>>>(p); else kv_read_kernel<true, false><<<grid, 256, 0, s>>>(p); }

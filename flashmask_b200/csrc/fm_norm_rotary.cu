@@ -472,7 +472,8 @@ static int norm_launch(const NormParams& p, bool back, cudaStream_t s) {
   if (back) {
     auto kern = norm_rotary_bwd_kernel<IS_BF16, IL, LPR>;
     constexpr int smem = 8 * NormStream<LPR>::BYTES + 8 * 2 * LPR * 16 * 4;
-    FM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> done{0};
+    FM_CUDA_TRY(allow_smem(kern, smem, done));
     kern<<<(unsigned)norm_bwd_grid(p), 256, smem, s>>>(p);
   } else {
     const int64_t jobs = (int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]);
