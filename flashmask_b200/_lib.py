@@ -30,7 +30,7 @@ class AttnArgs(C.Structure):
         ("ncols", C.c_int32), ("causal", C.c_int32), ("dtype", C.c_int32),
         ("mask_B", C.c_int32), ("tile_m", C.c_int32), ("tile_n", C.c_int32),
         ("deterministic", C.c_int32), ("bwd_flags", C.c_int32),
-        ("softmax_scale", C.c_float), ("reserved1", C.c_float),
+        ("softmax_scale", C.c_float), ("fwd_flags", C.c_int32),
         ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
         ("o", C.c_void_p), ("lse", C.c_void_p),
         ("mask", C.c_void_p), ("minmax", C.c_void_p), ("sink", C.c_void_p),

@@ -736,7 +736,8 @@ int bounded_wait_selftest_launch(uint64_t budget_ns, cudaStream_t s) {
 
 // Split plan of a call (SPLIT above): heads packed per query, parts, bytes of partial results.
 //
-// The plan is for calls without a mask tensor (the tiles a mask leaves are not known to the host).  Packing the heads
+// The plan is for calls without a mask tensor (the tiles a mask leaves are not known to the host), or with one that the caller
+// says to leave most tiles.  Packing the heads
 // of a group, dealing K tiles to several CTAs, and (where all rows of a block fit one sub-tile: p.alternate) letting
 // both sub-tiles take the tiles of a CTA in turn are each taken where an estimate of the launch says that it pays.
 // The estimate, in microseconds, is waves x (entry and exit + tiles per part + fp32 partial results of a part's rows)
@@ -749,7 +750,7 @@ int bounded_wait_selftest_launch(uint64_t budget_ns, cudaStream_t s) {
 struct FwdSplitPlan { int pack_log2, n_split; bool alternate; size_t bytes; };
 static FwdSplitPlan fwd_split_plan(const fm_attn_args* a) {
   FwdSplitPlan pl{0, 1, false, 0};
-  if (a->ncols != 0 || a->d > 128 || a->dv > 128) return pl;
+  if ((a->ncols != 0 && !(a->fwd_flags & FM_FWD_MASK_DENSE)) || a->d > 128 || a->dv > 128) return pl;
   const int G = a->Hq / a->Hkv, n_sm = sm_count(), tiles = (a->Sk + 127) / 128;
   const bool small = a->d <= 64 && a->dv <= 64;
   const double entry = small ? 4.9 : 5.7, in_turn = small ? 0.59 : 0.68, partial = small ? 4.5 : 10.0, merge = small ? 3.8 : 2.2;

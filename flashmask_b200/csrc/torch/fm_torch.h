@@ -22,10 +22,12 @@ Tensor rows(const Tensor& t);
 void strides(int64_t* out, const Tensor& t);
 // fp32 [Hq] on q's device; undefined stays undefined.
 Tensor sink_fp32(const Tensor& sink, const Tensor& q);
-// flashmask_attention: (out, lse).
-std::pair<Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& idx,
-                                    const std::optional<Tensor>& sink, std::optional<double> scale, bool causal,
-                                    int deterministic);
+// Arguments of a call without the launch tables: inputs, output, LSE; and its mask.
+fm_attn_args base_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, bool causal,
+                       double scale, const Tensor& sink32);
+void set_mask(fm_attn_args* a, const Tensor& idx, const Tensor& minmax, int tile_m, int tile_n);
+// The per-K-tile reductions of a mask.
+Tensor scan_mask(const Tensor& idx, int Sq, bool causal, int tile_m, int tile_n, void* stream);
 // The operators around attention (fm_torch_cache.cpp).
 void register_cache(pybind11::module_& m);
 

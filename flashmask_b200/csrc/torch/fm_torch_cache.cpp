@@ -281,7 +281,20 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
     fm_kv_args r = a;
     r.S = (int)cols; r.start = shift.data_ptr<int>(); r.k_out = k.data_ptr(); r.v_out = v.data_ptr();
     check(fm_kv_read(&f, &r, stream), "fm_kv_read");
-    return attention(query.detach(), k, v, bounds, sink32.defined() ? std::optional<Tensor>(sink32) : std::nullopt, scale, causal, 0);
+    const Tensor q = rows(query), out = fresh({B, S, Hq, f.dv}, q.scalar_type(), ck), lse = fresh({B, Hq, S}, at::kFloat, ck);
+    int tm = 0, tn = 0;
+    check(fm_fwd_tile_shape(f.d, f.dv, &tm, &tn), "fm_fwd_tile_shape");
+    const Tensor minmax = scan_mask(bounds, (int)S, causal, tm, tn, stream);
+    fm_attn_args x = base_args(q, k, v, out, lse, causal, scale, sink32);
+    set_mask(&x, bounds, minmax, tm, tn);
+    x.fwd_flags = FM_FWD_MASK_DENSE;
+    Tensor ws;
+    if ((x.workspace_bytes = fm_fwd_workspace_bytes(&x)) != 0) {
+      ws = fresh({(int64_t)x.workspace_bytes}, at::kByte, ck);
+      x.workspace = ws.data_ptr();
+    }
+    check(fm_fwd(&x, stream), "fm_fwd");
+    return {out, lse};
   }
   const Tensor q = vec_rows(query);
   const Tensor out = fresh({B, S, Hq, f.dv}, q.scalar_type(), ck), lse = fresh({B, Hq, S}, at::kFloat, ck);

@@ -136,7 +136,7 @@ typedef struct fm_attn_args {
   int32_t bwd_flags;      /* backward only, one-kernel variant: FM_BWD_* bits below, 0 = a
                              self-contained call                               */
   float softmax_scale;
-  float reserved1;
+  int32_t fwd_flags;      /* fm_fwd, fm_fwd_workspace_bytes: FM_FWD_* bits below       */
   const void* q; const void* k; const void* v;
   void* o; float* lse;
   const int32_t* mask;   /* [mask_B,Hm,Sk,ncols] or NULL                    */
@@ -162,6 +162,11 @@ typedef struct fm_attn_args {
   const int32_t* dq_order;   /* FM_ORDER_BWD_DQ, walked by fm_bwd                */
   const int32_t* dkdv_order; /* FM_ORDER_BWD_DKDV, walked by fm_bwd              */
 } fm_attn_args;
+
+/* The mask hides little of what the causal triangle leaves (padding, a window that is not much shorter than the keys):
+ * a call with few query rows may deal its K tiles to several CTAs as one without a mask does, and then takes no launch
+ * table.  Results are the same up to rounding. */
+#define FM_FWD_MASK_DENSE 1
 
 /* Tile shape (rows of Q, columns of K per tile) the forward / backward kernel
  * variant for (d, dv) classifies and skips on; `minmax` must be prepared with
