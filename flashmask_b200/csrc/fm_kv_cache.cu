@@ -15,10 +15,11 @@ struct KvWriteParams {
   int B, S;
 };
 
-// The part of 256 threads that walks rows of `upr` units of 8 values: thread = unit `col` of rows row0, row0 + step, ..
+// The part of a CTA's threads that walks rows of `upr` units of 8 values: thread = unit `col` of rows row0, row0 + step, ..
 struct RowWalk { int row0, step, col; };
+template <int THREADS>
 __device__ __forceinline__ RowWalk row_walk(int upr) {
-  const int step = 256 / upr, row0 = threadIdx.x / upr;
+  const int step = THREADS / upr, row0 = threadIdx.x / upr;
   return {row0 < step ? row0 : INT_MAX / 2, step, (int)threadIdx.x - row0 * upr};
 }
 
@@ -28,9 +29,10 @@ __device__ __forceinline__ RowWalk row_walk(int upr) {
 // A page that held tokens before (the write starts inside it) keeps its scale or grows it; where it grows, the payload
 // of the earlier tokens is rounded on the new grid.  Slots behind the last new token are left as they are.
 // VEC = units of 8 values that a thread holds.
-template <bool IS_BF16, bool INT8, int VEC>
-__global__ void __launch_bounds__(256, VEC <= 4 ? 5 : (VEC <= 8 ? 2 : 1)) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
-  __shared__ uint32_t s_max[8];
+template <bool IS_BF16, bool INT8, int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, VEC <= 4 ? 1280 / THREADS : (VEC <= 8 ? 2 : 1)) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ uint32_t s_max[WARPS];
   const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, P = 1 << p.g.page_log2;
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int start = p.start[b];
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(256, VEC <= 4 ? 5 : (VEC <= 8 ? 2 : 1)) kv_wri
   const int page = kv_page(p.g, p.table + b * p.g.table_stride, base);
   if (page < 0) return;
   const int w = p.width[which];
-  const RowWalk at = row_walk(w >> 3);
+  const RowWalk at = row_walk<THREADS>(w >> 3);
   const int lo = max(first - base, 0), hi = min(last - base + 1, P);       // slots [lo, hi) are new
   uint8_t* pay = p.pay[which] + ((size_t)page * p.g.Hkv + h) * P * w + at.col * 8;
   float* scale = p.scale[which] + (size_t)page * p.g.Hkv + h;
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(256, VEC <= 4 ? 5 : (VEC <= 8 ? 2 : 1)) kv_wri
     if ((threadIdx.x & 31) == 0) s_max[warp] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v = max(v, s_max[i]);
+    for (int i = 0; i < WARPS; ++i) v = max(v, s_max[i]);
     return v;
   };
   top = largest(top);
@@ -136,51 +138,58 @@ struct KvReadParams {
 };
 
 // dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  One CTA = the rows in one page of one kv
-// head, K or V, as in the write: the page and its scale are looked up once, and a thread has READ_ILP units of 8 bytes
-// in flight.  Bound by HBM: 3 bytes a value.
+// head, K and V: the page and its scales are looked up once, and a thread has READ_ILP units of 8 bytes of each in flight.
+// Bound by HBM: 3 bytes a value.
 constexpr int READ_ILP = 4;
 template <bool IS_BF16, bool INT8>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadParams p) {
-  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, w = p.width[which], P = 1 << p.g.page_log2;
+  const int b = blockIdx.z, h = blockIdx.y, P = 1 << p.g.page_log2;
   const int64_t start = p.start[b], base = ((start >> p.g.page_log2) + blockIdx.x) << p.g.page_log2;      // (rounds down below 0 too)
-  if (base >= start + p.S) return;
   const int len = kv_len(p.g, p.seqlens[b]);
+  if (base >= start + p.S) return;
   const int page = base >= 0 && base < len ? kv_page(p.g, p.table + b * p.g.table_stride, (int)base) : -1;
   const int lo = base < start ? (int)(start - base) : 0, hi = (int)min((int64_t)P, start + p.S - base);    // slots that are asked for
   const int valid = page >= 0 ? (int)min((int64_t)P, len - base) : 0;                                      // slots that hold tokens
-  const RowWalk at = row_walk(w >> 3);
-  const uint8_t* pay = p.pay[which];
-  float scale = 0.f;
-  if (page >= 0) {
-    const size_t ph = (size_t)page * p.g.Hkv + h;
-    pay += ph * P * w + at.col * 8;
-    scale = __ldg(p.scale[which] + ph);
+  const size_t ph = (size_t)max(page, 0) * p.g.Hkv + h;
+  const RowWalk at[2] = {row_walk<256>(p.width[0] >> 3), row_walk<256>(p.width[1] >> 3)};
+  float scale[2];
+  const uint8_t* pay[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    scale[x] = page >= 0 ? __ldg(p.scale[x] + ph) : 0.f;
+    pay[x] = p.pay[x] + ph * P * p.width[x] + at[x].col * 8;
   }
-  const int64_t out_row = (int64_t)p.g.Hkv * w;
-  uint16_t* dst = p.dst[which] + ((int64_t)b * p.S + (base - start)) * out_row + h * w + at.col * 8;
-  for (int row0 = lo + at.row0; row0 < hi; row0 += READ_ILP * at.step) {
-    uint2 v[READ_ILP];
+  for (int row0 = lo; row0 < hi; row0 += READ_ILP * min(at[0].step, at[1].step)) {
+    uint2 v[2][READ_ILP];
+    const int upto = min(hi, row0 + READ_ILP * min(at[0].step, at[1].step));
 #pragma unroll
-    for (int i = 0; i < READ_ILP; ++i) {
-      const int row = row0 + i * at.step;
-      v[i] = row < hi && row < valid ? __ldcs(reinterpret_cast<const uint2*>(pay + row * w)) : make_uint2(0, 0);
-    }
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int i = 0; i < READ_ILP; ++i) {
-      const int row = row0 + i * at.step;
-      if (row >= hi) break;
-      float a[4], c[4];
-      payload_f32<INT8>(v[i].x, a);
-      payload_f32<INT8>(v[i].y, c);
-      const float sc = row < valid ? scale : 0.f;                // (a NaN scale is no token's)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j] *= sc; c[j] *= sc;
-        // the 8-bit grid reaches a little beyond fp16; NaN passes
-        if (!IS_BF16) { if (fabsf(a[j]) > 65504.f) a[j] = copysignf(65504.f, a[j]); if (fabsf(c[j]) > 65504.f) c[j] = copysignf(65504.f, c[j]); }
+      for (int i = 0; i < READ_ILP; ++i) {
+        const int row = row0 + at[x].row0 + i * at[x].step;
+        v[x][i] = row < upto && row < valid ? __ldcs(reinterpret_cast<const uint2*>(pay[x] + row * p.width[x])) : make_uint2(0, 0);
       }
-      *reinterpret_cast<uint4*>(dst + row * out_row) = make_uint4(pack2<IS_BF16>(a[0], a[1]), pack2<IS_BF16>(a[2], a[3]),
-                                                                  pack2<IS_BF16>(c[0], c[1]), pack2<IS_BF16>(c[2], c[3]));
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int64_t out_row = (int64_t)p.g.Hkv * p.width[x];
+      uint16_t* dst = p.dst[x] + ((int64_t)b * p.S + (base - start)) * out_row + h * p.width[x] + at[x].col * 8;
+#pragma unroll
+      for (int i = 0; i < READ_ILP; ++i) {
+        const int row = row0 + at[x].row0 + i * at[x].step;
+        if (row >= upto) break;
+        float a[4], c[4];
+        payload_f32<INT8>(v[x][i].x, a);
+        payload_f32<INT8>(v[x][i].y, c);
+        const float sc = row < valid ? scale[x] : 0.f;            // (a NaN scale is no token's)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          a[j] *= sc; c[j] *= sc;
+          // the 8-bit grid reaches a little beyond fp16; NaN passes
+          if (!IS_BF16) { if (fabsf(a[j]) > 65504.f) a[j] = copysignf(65504.f, a[j]); if (fabsf(c[j]) > 65504.f) c[j] = copysignf(65504.f, c[j]); }
+        }
+        *reinterpret_cast<uint4*>(dst + row * out_row) = make_uint4(pack2<IS_BF16>(a[0], a[1]), pack2<IS_BF16>(a[2], a[3]),
+                                                                    pack2<IS_BF16>(c[0], c[1]), pack2<IS_BF16>(c[2], c[3]));
+      }
     }
   }
 }
@@ -251,11 +260,15 @@ static unsigned pages_of(int S, int page_size) { return (unsigned)(((int64_t)S +
 
 template <bool IS_BF16, bool INT8>
 static int launch_write(const KvWriteParams& p, int page_size, int width_max, cudaStream_t s) {
-  const int step = 256 / (width_max / 8), vec = (std::min(page_size, p.S) + step - 1) / step;      // <= 16
   const dim3 grid(pages_of(p.S, page_size), 2 * p.g.Hkv, p.B);
-#define FM_KV_WRITE(N) if (vec <= N) { kv_write_kernel<IS_BF16, INT8, N><<<grid, 256, 0, s>>>(p); }
-  FM_KV_WRITE(1) else FM_KV_WRITE(2) else FM_KV_WRITE(4) else FM_KV_WRITE(8) else FM_KV_WRITE(16)
-#undef FM_KV_WRITE
+  const int upr = width_max / 8, rows = std::min(page_size, p.S), vec = (rows + 256 / upr - 1) / (256 / upr);      // <= 16
+  // (a few tokens: a CTA of 64 threads has a unit for each, and 2048 of them fit the chip at once)
+  if (rows <= 64 / upr) kv_write_kernel<IS_BF16, INT8, 1, 64><<<grid, 64, 0, s>>>(p);
+  else if (vec <= 1) kv_write_kernel<IS_BF16, INT8, 1, 256><<<grid, 256, 0, s>>>(p);
+  else if (vec <= 2) kv_write_kernel<IS_BF16, INT8, 2, 256><<<grid, 256, 0, s>>>(p);
+  else if (vec <= 4) kv_write_kernel<IS_BF16, INT8, 4, 256><<<grid, 256, 0, s>>>(p);
+  else if (vec <= 8) kv_write_kernel<IS_BF16, INT8, 8, 256><<<grid, 256, 0, s>>>(p);
+  else kv_write_kernel<IS_BF16, INT8, 16, 256><<<grid, 256, 0, s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   return FM_OK;
@@ -307,7 +320,7 @@ extern "C" FM_API int fm_kv_read(const fm_kv_cache* c, const fm_kv_args* a, void
   p.width[0] = c->d; p.width[1] = c->dv;
   p.table = a->page_table; p.start = a->start; p.seqlens = a->seqlens;
   p.B = a->B; p.S = a->S;
-  const dim3 grid(pages_of(a->S, c->page_size), 2 * c->Hkv, a->B);
+  const dim3 grid(pages_of(a->S, c->page_size), c->Hkv, a->B);
   const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
   cudaStream_t s = (cudaStream_t)stream;
   if (bf) { if (i8) kv_read_kernel<true, true><<<grid, 256, 0, s>>>(p); else kv_read_kernel<true, false><<<grid, 256, 0, s>>>(p); }
