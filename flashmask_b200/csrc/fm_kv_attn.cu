@@ -51,9 +51,9 @@ struct KvCfg {
   static constexpr int STAGES = (CTAS == 1 ? 192 : (CTAS == 2 ? (NT > 2 ? 80 : 96) : (CTAS == 3 ? 64 : 48))) * 1024 / (KV_WARPS * STAGE);
   static constexpr int RING = KV_WARPS * STAGES * STAGE;
   static constexpr int ROWS = 8 * NT, DV = 8 * VC, MT = VC / 2;  // MT row tiles of O^T
-  static constexpr int JOIN = STAGE / (MT * 512) < NT ? STAGE / (MT * 512) : NT;    // column tiles whose O fits a stage
+  static constexpr int FIT = STAGE / (MT * 512), JOIN = FIT >= NT ? NT : (NT % 2 == 0 && FIT >= 2 ? 2 : 1);    // column tiles of O joined together: a stage holds them
   static constexpr int Q = NT * DK * 4 * 32 * 8;                 // Q^T fragments
-  static constexpr int FIXED = RING + Q + KV_WARPS * KV_INFO * 16 + 2 * KV_WARPS * ROWS * 4 + ROWS * 12;   // .., info, m, l, limits and scales
+  static constexpr int FIXED = RING + Q + KV_WARPS * KV_INFO * 16 + 2 * KV_WARPS * ROWS * 4 + ROWS * 20;   // .., info, m, l, limits, scales, totals
   static_assert(STAGES >= 2 && 2 * STAGES <= KV_INFO - 32, "a block is copied while another is used");
   static_assert(JOIN > 0 && NT % JOIN == 0 && NT <= KV_WARPS, "O fits the stage of the last block; a warp for every tile of queries");
 };
@@ -124,15 +124,24 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
   float* s_l = s_m + KV_WARPS * ROWS;                 // [warps][ROWS]
   int2* s_lim = reinterpret_cast<int2*>(s_l + KV_WARPS * ROWS);             // [ROWS] keys that a row sees
   float* s_f = reinterpret_cast<float*>(s_lim + ROWS);                      // [ROWS] scale of a row of q
-  int* s_pre = reinterpret_cast<int*>(s_f + ROWS);    // [B + 1] first unit of every sequence
+  float2* s_tot = reinterpret_cast<float2*>(s_f + ROWS);                    // [ROWS] maximum and sum of a row
+  int* s_pre = reinterpret_cast<int*>(s_tot + ROWS);  // [B + 1] first unit of every sequence
   __shared__ int s_scan[KV_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int d = FULL ? DK * 64 : p.d, dv = FULL ? VC * 8 : p.dv;
   grid_dep_trigger();                                 // (the merge waits for this kernel's end before it reads anything)
   const int items = p.g.Hkv * p.row_tiles;            // of one sequence
-  // sequences b0 .. of this thread; most calls have one at most
-  const int per = (p.B + KV_WARPS * 32 - 1) / (KV_WARPS * 32), b0 = tid * per, b1 = min(b0 + per, p.B);
-  {
+  if (p.B <= 32) {
+    // (every warp for itself, without a barrier)
+    int x = lane < p.B ? kv_units(kv_range(p, lane)) * items : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+    s_pre += warp * 33;
+    if (lane < p.B) s_pre[lane + 1] = x;
+    if (lane == 0) s_pre[0] = 0;
+    __syncwarp();
+  } else {
+    const int per = (p.B + KV_WARPS * 32 - 1) / (KV_WARPS * 32), b0 = tid * per, b1 = min(b0 + per, p.B);
     int mine = 0;
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) { s_pre[b] = mine; mine += kv_units(kv_range(p, b)) * items; }
@@ -249,6 +258,20 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
         }
       }
     __syncthreads();
+    if (tid < ROWS) {
+      // a row's maximum and sum over the warps, and every warp's weight in place of its maximum
+      float mk[KV_WARPS], lk[KV_WARPS], top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < KV_WARPS; ++k) { mk[k] = s_m[k * ROWS + tid]; lk[k] = s_l[k * ROWS + tid]; top = fmaxf(top, mk[k]); }
+#pragma unroll
+      for (int k = 0; k < KV_WARPS; ++k) {
+        const float w = mk[k] == -INFINITY ? (lk[k] == 0.f ? 0.f : 1.f) : fast_exp2(mk[k] - top);    // (l NaN without a maximum: kept)
+        s_m[k * ROWS + tid] = w;
+        sum += lk[k] * w;
+      }
+      s_tot[tid] = make_float2(top, sum);
+    }
+    __syncthreads();
     const bool whole = s.u0 == 0 && s.u1 == s.units;
     const int slot = 2 * blockIdx.x + (s.u0 > 0 ? 0 : 1);
 #pragma unroll
@@ -257,18 +280,11 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
 #pragma unroll
       for (int n = 0; n < JOIN; ++n) {
         const int nt = pass * JOIN + n;
-        float w[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int x = 0; x < KV_WARPS; ++x) top = fmaxf(top, s_m[x * ROWS + nt * 8 + 2 * t + j]);
-          w[j] = m[nt][j] == -INFINITY ? (l[nt][j] == 0.f ? 0.f : 1.f) : fast_exp2(m[nt][j] - top);    // (l NaN without a maximum: kept)
-        }
+        const float2 w = *reinterpret_cast<const float2*>(s_m + warp * ROWS + nt * 8 + 2 * t);
 #pragma unroll
         for (int jj = 0; jj < MT; ++jj)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s_o[warp * WARP_O + ((n * MT + jj) * 4 + c) * 32 + lane] = o[nt][jj][c] * w[c & 1];
+          for (int c = 0; c < 4; ++c) s_o[warp * WARP_O + ((n * MT + jj) * 4 + c) * 32 + lane] = o[nt][jj][c] * (c & 1 ? w.y : w.x);
       }
       __syncthreads();
       // thread = 4 neighbouring dims of a row
@@ -277,30 +293,24 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
         constexpr int CH = VC < 16 ? VC : 16;              // bytes of one chunk
         const int c8 = x / (DV / 4), dim = (x - c8 * (DV / 4)) * 4, chunk = dim / (8 * CH), in = dim - chunk * 8 * CH;
         const int gg = in / CH, byte = in - gg * CH + chunk * CH, col = pass * JOIN * 8 + c8, row = s.row0 + col, i = row / p.G;
-        if (i >= p.S) continue;
+        if (i >= p.S) break;                               // (rows go up with x)
         const float* src = s_o + ((c8 >> 3) * MT * 4 + (byte >> 1) * 4 + (c8 & 1)) * 32 + gg * 4 + ((c8 & 7) >> 1);
-        float v[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < KV_WARPS; ++k) {
-          top = fmaxf(top, s_m[k * ROWS + col]);
+        for (int k = 0; k < KV_WARPS; ++k)
 #pragma unroll
           for (int c = 0; c < 4; ++c) v[c] += src[k * WARP_O + (c >> 1) * 128 + (c & 1) * 64];
-        }
-#pragma unroll
-        for (int k = 0; k < KV_WARPS; ++k) {
-          const float mk = s_m[k * ROWS + col], lk = s_l[k * ROWS + col];
-          sum += mk == -INFINITY ? lk : lk * fast_exp2(mk - top);
-        }
+        float2 tot = s_tot[col];
         if (whole) {
           const int hq = s.h * p.G + row - i * p.G;
           if (p.sink) {
-            const float sk = p.sink[hq] * kLog2e, up = fmaxf(top, sk), z = top == -INFINITY ? 1.f : fast_exp2(top - up);
-            sum = sum * z + (sk == -INFINITY ? 0.f : fast_exp2(sk - up));
+            const float sk = p.sink[hq] * kLog2e, up = fmaxf(tot.x, sk), z = tot.x == -INFINITY ? 1.f : fast_exp2(tot.x - up);
+            tot.y = tot.y * z + (sk == -INFINITY ? 0.f : fast_exp2(sk - up));
             v[0] *= z; v[1] *= z; v[2] *= z; v[3] *= z;
-            top = up;
+            tot.x = up;
           }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          if (dim == 0) p.lse[((int64_t)s.b * p.Hq + hq) * p.S + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+          const float inv = tot.y == 0.f ? 0.f : 1.f / tot.y;
+          if (dim == 0) p.lse[((int64_t)s.b * p.Hq + hq) * p.S + i] = tot.y == 0.f ? -INFINITY : (tot.x + log2f(tot.y)) * kLn2;
           if (FULL || dim < dv) {
             const uint2 z = p.bf16 ? make_uint2(pack2<true>(v[0] * inv, v[1] * inv), pack2<true>(v[2] * inv, v[3] * inv))
                                    : make_uint2(pack2<false>(v[0] * inv, v[1] * inv), pack2<false>(v[2] * inv, v[3] * inv));
@@ -308,7 +318,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
           }
         } else {
           *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * ROWS + col) * DV + dim) = make_float4(v[0], v[1], v[2], v[3]);
-          if (dim == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * ROWS + col) * 2) = make_float2(top, sum);
+          if (dim == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * ROWS + col) * 2) = tot;
         }
       }
     }
@@ -587,13 +597,15 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
 
 // One CTA = one query row (of a kv head's rows) of one item; it joins the parts when the item was cut, which lie in
 // consecutive CTAs' slots.  Where the item was cut follows from the lengths, which are there before the parts are.  Every
-// warp computes all parts' weights, a lane each; the warps take the parts in turn and are joined in order.
-template <int DV, int ROWS>
-__global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p) {
-  constexpr int PER = DV / 32, AHEAD = 4;
+// warp computes all parts' weights, a lane each.  ONE: a row is a warp's (many rows of few parts), else a CTA's, whose
+// warps take the parts in turn and are joined in order.
+template <int DV, int ROWS, bool ONE>
+__global__ void __launch_bounds__(128) kv_attn_merge_kernel(const __grid_constant__ KvAttnParams p) {
+  constexpr int PER = DV / 32, AHEAD = 4, STEP = ONE ? 1 : 4;
   __shared__ float s_v[4][DV];
   __shared__ int s_sum[2][4];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, h = blockIdx.y, row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.z, h = blockIdx.y, row = ONE ? blockIdx.x * 4 + warp : blockIdx.x;
+  const int first = ONE ? 0 : warp;                       // of the parts of this warp
   const int items = p.g.Hkv * p.row_tiles, mine = kv_units(kv_range(p, b));
   int before = 0, all = 0;
   for (int x = threadIdx.x; x < p.B; x += 128) {
@@ -611,7 +623,7 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p
   const int64_t s0 = before + (int64_t)(h * p.row_tiles + tile) * mine, s1 = s0 + mine - 1;
   const int c0 = (int)(((s0 + 1) * n - 1) / total), c1 = (int)(((s1 + 1) * n - 1) / total);
   grid_dep_wait();
-  if (c0 == c1) return;                                   // done by one CTA
+  if (c0 == c1 || row >= p.S * p.G) return;               // done by one CTA; no row
   auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS + in_tile; };
   auto get_ml = [&](int c) {
     return c <= c1 ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot(c)) : make_float2(-INFINITY, 0.f);
@@ -620,10 +632,10 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p
   auto get_o = [&](int c) {                              // AHEAD parts of this warp, from c on
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const float* src = p.part_o + slot(c + 4 * a) * DV + lane * PER;
+      const float* src = p.part_o + slot(c + STEP * a) * DV + lane * PER;
 #pragma unroll
       for (int e = 0; e < PER; ++e) y[a][e] = 0.f;
-      if (c + 4 * a > c1) continue;
+      if (c + STEP * a > c1) continue;
       if constexpr (PER == 2) { const float2 q = __ldcg(reinterpret_cast<const float2*>(src)); y[a][0] = q.x; y[a][1] = q.y; }
       else {
 #pragma unroll
@@ -635,7 +647,7 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p
     }
   };
   float2 ml = get_ml(c0 + lane);
-  get_o(c0 + warp);
+  get_o(c0 + first);
   const int i = row / p.G, hq = h * p.G + row - i * p.G;
   const float sk = p.sink ? p.sink[hq] * kLog2e : -INFINITY;
   float top = fmaxf(sk, ml.x);
@@ -649,28 +661,36 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const KvAttnParams p
     if (base > c0) ml = get_ml(base + lane);
     const float w_mine = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);    // (l NaN without a maximum: kept)
     sum += ml.y * w_mine;
-    for (int x0 = warp; x0 < 32 && base + x0 <= c1; x0 += 4 * AHEAD) {
-      if (base + x0 > c0 + warp) get_o(base + x0);
+    for (int x0 = first; x0 < 32 && base + x0 <= c1; x0 += STEP * AHEAD) {
+      if (base + x0 > c0 + first) get_o(base + x0);
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
-        const float w = __shfl_sync(0xffffffffu, w_mine, x0 + 4 * a);
+        const float w = __shfl_sync(0xffffffffu, w_mine, x0 + STEP * a);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) v[e] += base + x0 + 4 * a <= c1 ? w * y[a][e] : 0.f;
+        for (int e = 0; e < PER; ++e) v[e] += base + x0 + STEP * a <= c1 ? w * y[a][e] : 0.f;
       }
     }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (sk != -INFINITY) sum += fast_exp2(sk - top);
-#pragma unroll
-  for (int x = 0; x < PER; ++x) s_v[warp][lane * PER + x] = v[x];
-  __syncthreads();
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (threadIdx.x == 0) p.lse[((int64_t)b * p.Hq + hq) * p.S + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-  for (int dim = threadIdx.x * 2; dim < p.dv; dim += 256) {
-    const float x = (s_v[0][dim] + s_v[1][dim] + s_v[2][dim] + s_v[3][dim]) * inv;
-    const float y = (s_v[0][dim + 1] + s_v[1][dim + 1] + s_v[2][dim + 1] + s_v[3][dim + 1]) * inv;
-    *reinterpret_cast<uint32_t*>(p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * p.dv + dim) = p.bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
+  if (lane == 0 && (ONE || warp == 0)) p.lse[((int64_t)b * p.Hq + hq) * p.S + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  uint16_t* out = p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * p.dv;
+  if constexpr (ONE) {
+    if (lane * PER < p.dv)
+#pragma unroll
+      for (int x = 0; x < PER; x += 2)
+        *reinterpret_cast<uint32_t*>(out + lane * PER + x) = p.bf16 ? pack2<true>(v[x] * inv, v[x + 1] * inv) : pack2<false>(v[x] * inv, v[x + 1] * inv);
+  } else {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) s_v[warp][lane * PER + x] = v[x];
+    __syncthreads();
+    for (int dim = threadIdx.x * 2; dim < p.dv; dim += 256) {
+      const float x = (s_v[0][dim] + s_v[1][dim] + s_v[2][dim] + s_v[3][dim]) * inv;
+      const float y2 = (s_v[0][dim + 1] + s_v[1][dim + 1] + s_v[2][dim + 1] + s_v[3][dim + 1]) * inv;
+      *reinterpret_cast<uint32_t*>(out + dim) = p.bf16 ? pack2<true>(x, y2) : pack2<false>(x, y2);
+    }
   }
 }
 
@@ -687,10 +707,10 @@ static KvAttnPlan kv_attn_plan(const fm_kv_cache* c, const fm_kv_args* a) {
   KvAttnPlan pl;
   const int rows = a->S * (a->Hq / c->Hkv);
   pl.vc = c->dv <= 64 && c->d <= 64 ? 8 : (c->dv <= 128 ? 16 : 32);
-  pl.nt = rows <= 8 || pl.vc == 32 ? 1 : (rows <= 16 || c->d > 128 ? 2 : 4);
+  pl.nt = rows <= 8 || pl.vc == 32 ? 1 : (rows <= 16 || c->d > 128 ? 2 : (rows <= 24 ? 3 : 4));
   pl.n_cta = sm_count() * (pl.vc > 16 ? KvCfg<4, 32, 1>::CTAS : c->d > 128 ? KvCfg<3, 16, 1>::CTAS
-             : pl.vc == 16 ? (pl.nt == 1 ? KvCfg<2, 16, 1>::CTAS : pl.nt == 2 ? KvCfg<2, 16, 2>::CTAS : KvCfg<2, 16, 4>::CTAS)
-                           : (pl.nt == 1 ? KvCfg<1, 8, 1>::CTAS : pl.nt == 2 ? KvCfg<1, 8, 2>::CTAS : KvCfg<1, 8, 4>::CTAS));
+             : pl.vc == 16 ? (pl.nt == 1 ? KvCfg<2, 16, 1>::CTAS : pl.nt == 2 ? KvCfg<2, 16, 2>::CTAS : pl.nt == 3 ? KvCfg<2, 16, 3>::CTAS : KvCfg<2, 16, 4>::CTAS)
+                           : (pl.nt == 1 ? KvCfg<1, 8, 1>::CTAS : pl.nt == 2 ? KvCfg<1, 8, 2>::CTAS : pl.nt == 3 ? KvCfg<1, 8, 3>::CTAS : KvCfg<1, 8, 4>::CTAS));
   pl.bytes = (size_t)2 * pl.n_cta * pl.nt * 8 * (8 * pl.vc + 2) * sizeof(float);
   return pl;
 }
@@ -699,13 +719,18 @@ template <int DK, int VC, int NT, bool INT8, bool FULL>
 static int launch_kv_attn(const KvAttnParams& p, cudaStream_t s) {
   using Cfg = KvCfg<DK, VC, NT>;
   auto kern = kv_attn_kernel<DK, VC, NT, INT8, FULL>;
-  const size_t smem = Cfg::FIXED + (size_t)(p.B + 1) * 4;
+  const size_t smem = Cfg::FIXED + (size_t)std::max(p.B + 1, KV_WARPS * 33) * 4;      // first units of the sequences
   static std::atomic<uint64_t> done{0};
   FM_CUDA_TRY(allow_smem(kern, Cfg::FIXED + (KV_MAX_B + 1) * 4, done));
   kern<<<p.n_cta, KV_WARPS * 32, smem, s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
-  FM_CUDA_TRY(launch_dependent(kv_attn_merge_kernel<8 * VC, 8 * NT>, dim3(p.S * p.G, p.g.Hkv, p.B), dim3(128), 0, s, p));
+  // (a row of up to 8 parts is one warp's)
+  const int rows = p.S * p.G;
+  if ((int64_t)p.B * p.g.Hkv * p.row_tiles * 8 >= p.n_cta)
+    FM_CUDA_TRY(launch_dependent(kv_attn_merge_kernel<8 * VC, 8 * NT, true>, dim3((rows + 3) / 4, p.g.Hkv, p.B), dim3(128), 0, s, p));
+  else
+    FM_CUDA_TRY(launch_dependent(kv_attn_merge_kernel<8 * VC, 8 * NT, false>, dim3(rows, p.g.Hkv, p.B), dim3(128), 0, s, p));
   count_launches(1);
   return FM_OK;
 }
@@ -715,7 +740,7 @@ static int launch_kv_attn_rows(const KvAttnParams& p, int nt, cudaStream_t s) {
   if (nt == 1 || VC > 16) return launch_kv_attn<DK, VC, 1, INT8, FULL>(p, s);
   if constexpr (VC <= 16) {
     if (nt == 2 || DK > 2) return launch_kv_attn<DK, VC, 2, INT8, FULL>(p, s);
-    if constexpr (DK <= 2) return launch_kv_attn<DK, VC, 4, INT8, FULL>(p, s);
+    if constexpr (DK <= 2) return nt == 3 ? launch_kv_attn<DK, VC, 3, INT8, FULL>(p, s) : launch_kv_attn<DK, VC, 4, INT8, FULL>(p, s);
   }
   return FM_ERR_UNSUPPORTED;
 }
