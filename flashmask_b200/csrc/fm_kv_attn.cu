@@ -85,17 +85,24 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnParams& p, int b) {
   r.n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   r.p0 = r.len - r.n;
   r.hi = r.n > 0 ? r.len : 0;
-  r.lo = p.window > 0 ? min(max((int64_t)r.p0 - p.window + 1, (int64_t)0), (int64_t)r.hi) & ~(KV_BLOCK - 1) : 0;
+  r.lo = p.window > 0 ? min(max(r.p0 - p.window + 1, 0), r.hi) & ~(KV_BLOCK - 1) : 0;      // (the host keeps window and S below 2^30)
   return r;
 }
 __device__ __forceinline__ int kv_units(const KvRange& r) { return max(1, (r.hi - r.lo + KV_UNIT - 1) / KV_UNIT); }
+
+// The units are dealt to n CTAs, the first total % n of which get one more.
+__device__ __forceinline__ int kv_first_unit(int total, int n, int c) { return total / n * c + min(c, total % n); }
+__device__ __forceinline__ int kv_cta_of(int total, int n, int unit) {
+  const int q = total / n, r = total % n;
+  return unit < r * (q + 1) ? unit / (q + 1) : r + (unit - r * (q + 1)) / q;
+}
 
 // Keys [lo, hi) that query row i sees; a row that is none sees nothing.
 __device__ __forceinline__ void row_range(const KvAttnParams& p, const KvRange& r, int i, int& lo, int& hi) {
   lo = 0; hi = 0;
   if (i >= r.n) return;
   hi = p.causal ? max(r.p0 + i + 1, 0) : r.len;
-  if (p.window > 0) lo = (int)max((int64_t)0, (int64_t)r.p0 + i + 1 - p.window);
+  if (p.window > 0) lo = max(0, r.p0 + i + 1 - p.window);
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
   }
   const int total = s_pre[p.B], n_cta = min(p.n_cta, total);            // (never a CTA without a unit between two with one)
   if (blockIdx.x >= n_cta) return;
-  const int u_begin = (int)((int64_t)total * blockIdx.x / n_cta), n_units = (int)((int64_t)total * (blockIdx.x + 1) / n_cta) - u_begin;
+  const int u_begin = kv_first_unit(total, n_cta, blockIdx.x), n_units = total / n_cta + (blockIdx.x < total % n_cta ? 1 : 0);
 
   // The part of the item of unit u that this CTA has from u on.
   auto segment = [&](int u) {
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
     const int in_seq = u - s_pre[b], item = in_seq / s.units;
     s.u0 = in_seq - item * s.units;
     s.u1 = min(s.units, s.u0 + u_begin + n_units - u);
-    s.h = item / p.row_tiles;
+    s.h = p.row_tiles == 1 ? item : item / p.row_tiles;
     s.row0 = (item - s.h * p.row_tiles) * ROWS;
     s.key0 = s.r.lo + s.u0 * KV_UNIT;
     return s;
@@ -617,11 +624,10 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const __grid_constan
   for (int o = 16; o; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); }
   if (lane == 0) { s_sum[0][warp] = all; s_sum[1][warp] = before; }
   __syncthreads();
-  const int64_t total = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3], n = min((int64_t)p.n_cta, total);
+  const int total = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3], n = min(p.n_cta, total);
   before = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
   const int tile = row / ROWS, in_tile = row - tile * ROWS;
-  const int64_t s0 = before + (int64_t)(h * p.row_tiles + tile) * mine, s1 = s0 + mine - 1;
-  const int c0 = (int)(((s0 + 1) * n - 1) / total), c1 = (int)(((s1 + 1) * n - 1) / total);
+  const int s0 = before + (h * p.row_tiles + min(tile, p.row_tiles - 1)) * mine, c0 = kv_cta_of(total, n, s0), c1 = kv_cta_of(total, n, s0 + mine - 1);
   grid_dep_wait();
   if (c0 == c1 || row >= p.S * p.G) return;               // done by one CTA; no row
   auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS + in_tile; };
@@ -705,7 +711,7 @@ constexpr int KV_MAX_B = 1024;                      // first units of the sequen
 struct KvAttnPlan { int vc, nt, n_cta; size_t bytes; };
 static KvAttnPlan kv_attn_plan(const fm_kv_cache* c, const fm_kv_args* a) {
   KvAttnPlan pl;
-  const int rows = a->S * (a->Hq / c->Hkv);
+  const int64_t rows = (int64_t)a->S * (a->Hq / c->Hkv);
   pl.vc = c->dv <= 64 && c->d <= 64 ? 8 : (c->dv <= 128 ? 16 : 32);
   pl.nt = rows <= 8 || pl.vc == 32 ? 1 : (rows <= 16 || c->d > 128 ? 2 : (rows <= 24 ? 3 : 4));
   pl.n_cta = sm_count() * (pl.vc > 16 ? KvCfg<4, 32, 1>::CTAS : c->d > 128 ? KvCfg<3, 16, 1>::CTAS
@@ -782,7 +788,7 @@ extern "C" FM_API int fm_kv_attention(const fm_kv_cache* c, const fm_kv_args* a,
   const KvAttnPlan pl = kv_attn_plan(c, a);
   const int64_t G = a->Hq / c->Hkv, rows = a->S * G, tiles = (rows + pl.nt * 8 - 1) / (pl.nt * 8);
   const int64_t units = ((int64_t)a->max_pages * c->page_size + 31) / KV_UNIT + 1;
-  FM_REQUIRE(rows < INT_MAX && units * tiles <= (INT_MAX - 1) / c->Hkv / a->B, FM_ERR_UNSUPPORTED, "fm_kv_attention: too many rows and keys for one call");
+  FM_REQUIRE(rows < 1 << 30 && units * tiles <= (INT_MAX - 1) / c->Hkv / a->B, FM_ERR_UNSUPPORTED, "fm_kv_attention: too many rows and keys for one call");
   FM_REQUIRE((int64_t)c->num_pages * c->Hkv * c->page_size / 16 < INT_MAX, FM_ERR_UNSUPPORTED, "fm_kv_attention: a cache of 2^31 groups of 16 tokens");
   FM_REQUIRE(a->workspace && a->workspace_bytes >= pl.bytes && ((uintptr_t)a->workspace & 15) == 0, FM_ERR_WORKSPACE,
              "fm_kv_attention: workspace of %zu bytes, %zu needed", a->workspace_bytes, pl.bytes);
@@ -790,7 +796,7 @@ extern "C" FM_API int fm_kv_attention(const fm_kv_cache* c, const fm_kv_args* a,
   p.table = a->page_table; p.seqlens = a->seqlens; p.lengths = a->lengths;
   p.q = (const uint16_t*)a->q; p.o = (uint16_t*)a->o; p.lse = a->lse; p.sink = a->sink;
   p.B = a->B; p.S = a->S; p.Hq = a->Hq; p.G = (int)G; p.d = c->d; p.dv = c->dv;
-  p.causal = a->causal; p.window = a->window; p.bf16 = a->dtype == FM_DTYPE_BF16;
+  p.causal = a->causal; p.window = std::min(a->window, 1 << 30); p.bf16 = a->dtype == FM_DTYPE_BF16;
   p.row_tiles = (int)tiles;
   p.scale_log2 = a->softmax_scale * kLog2e;
   p.n_cta = pl.n_cta;

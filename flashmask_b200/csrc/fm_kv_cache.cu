@@ -252,6 +252,7 @@ int kv_geometry(const fm_kv_cache* c, const fm_kv_args* a, KvGeom* g) {
   FM_REQUIRE(a->table_stride >= a->max_pages || a->B <= 1, FM_ERR_INVALID_ARGUMENT, "kv cache: table_stride below max_pages");
   g->num_pages = c->num_pages; g->page_log2 = page_log2_of(c->page_size); g->Hkv = c->Hkv;
   g->max_pages = a->max_pages; g->table_stride = a->table_stride;
+  g->cap = a->max_pages * c->page_size;
   return FM_OK;
 }
 

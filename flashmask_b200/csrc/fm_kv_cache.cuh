@@ -16,6 +16,7 @@ namespace fm {
 
 struct KvGeom {
   int num_pages, page_log2, Hkv, max_pages;
+  int cap;                       // positions of a row of the page table
   int64_t table_stride;
 };
 
@@ -31,10 +32,7 @@ __host__ __device__ __forceinline__ int kv_page(const KvGeom& g, const int32_t* 
 }
 
 // Length of a sequence as the kernels use it: never beyond its page table.
-__host__ __device__ __forceinline__ int kv_len(const KvGeom& g, int len) {
-  const int64_t cap = (int64_t)g.max_pages << g.page_log2;
-  return len < 0 ? 0 : (len > cap ? (int)cap : len);
-}
+__host__ __device__ __forceinline__ int kv_len(const KvGeom& g, int len) { return len < 0 ? 0 : (len > g.cap ? g.cap : len); }
 
 constexpr int kCacheMinExp = -64;
 template <bool INT8> constexpr int kCacheMaxExp = INT8 ? 121 : 119;     // largest e with a finite 127 * 2^e | 448 * 2^e
