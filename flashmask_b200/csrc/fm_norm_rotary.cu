@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_co
   int lo, hi;
   slot_offsets<INTERLEAVED>(s, p.rot, lo, hi);
   float* sums = reinterpret_cast<float*>(smem + 8 * Stream::BYTES);
-  grid_dep_trigger();                                            // (the sum over the CTAs waits for this kernel's end)
+  if (p.part) grid_dep_trigger();                                // (the sum over the CTAs follows, and waits for this kernel's end)
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     const int step = gridDim.x * 8;

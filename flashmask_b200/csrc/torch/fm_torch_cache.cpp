@@ -241,8 +241,13 @@ std::pair<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Tens
 }
 
 // Rows (queries x heads of a group) up to which the cache is read by the kernel for few rows.  Beyond, the tokens are
-// read back once into dense 16-bit tensors and the dense forward, which feeds the tensor cores, takes the call.
-constexpr int64_t kFewRows = 64;
+// read back once into dense 16-bit tensors and the dense forward, which feeds the tensor cores, takes the call.  Measured, 32 / 8
+// heads, d = 128: 64 rows 37 us and 68 rows 48 us for 16384 keys (128 rows: 54), 54 and 78 us for 8 x 4096 (82), 118 and 165
+// us for 64 x 1024, where the kernel's time goes with the number of 32-row tiles and the other's hardly with the rows.
+constexpr int64_t kFewRows = 96;
+// Without an upper bound of the lengths the dense tensors cover the whole page table, which may be far wider than the
+// sequences are long: beyond this many bytes the kernel for few rows, which needs none, keeps the call.
+constexpr int64_t kNoBound = (int64_t)1 << 40, kMostDense = (int64_t)2 << 30;
 
 std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs,
                                        const Tensor& table, const Tensor& seqlens, const std::optional<Tensor>& lengths,
@@ -257,6 +262,7 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
   if (sink) require(sink->numel() == query.size(2), "sink must have one logit per q head");
   TORCH_CHECK_VALUE(window >= 0 && (causal || window == 0), "window_size needs causal=True and at least one token");
   no_gradient(query, "kv_cache_attention");
+  if (sink) no_gradient(*sink, "kv_cache_attention");
   const c10::cuda::CUDAGuard guard(ck.device());
   Tensor keep[3];
   const int64_t B = query.size(0), S = query.size(1), Hq = query.size(2);
@@ -271,17 +277,18 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
   a.softmax_scale = (float)scale;
   void* stream = stream_of(ck);
   const Tensor sink32 = sink ? sink_fp32(*sink, query) : Tensor();
-  if (S * (Hq / f.Hkv) > kFewRows && B > 0) {
-    int64_t cols = std::min<int64_t>(max_seqlen, (int64_t)a.max_pages * f.page_size);
-    // (with rows that do not count the real ones stand up to S columns further left)
-    cols = std::max<int64_t>(lengths ? cols + S : cols, S);
+  // columns of the dense tensors (with rows that do not count the real ones stand up to S columns further left)
+  int64_t cols = std::min<int64_t>(max_seqlen, (int64_t)a.max_pages * f.page_size);
+  cols = std::max<int64_t>(lengths ? cols + S : cols, S);
+  const bool bounded = max_seqlen < kNoBound || B * cols * f.Hkv * (f.d + f.dv) * 2 <= kMostDense;
+  if (S * (Hq / f.Hkv) > kFewRows && B > 0 && bounded) {
     const Tensor shift = fresh({B}, at::kInt, ck), bounds = fresh({B, 1, cols, causal ? 1 : 2}, at::kInt, ck);
     check(fm_kv_bounds(&f, &a, (int)cols, shift.data_ptr<int>(), bounds.data_ptr<int>(), stream), "fm_kv_bounds");
     const Tensor k = fresh({B, cols, f.Hkv, f.d}, query.scalar_type(), ck), v = fresh({B, cols, f.Hkv, f.dv}, query.scalar_type(), ck);
     fm_kv_args r = a;
     r.S = (int)cols; r.start = shift.data_ptr<int>(); r.k_out = k.data_ptr(); r.v_out = v.data_ptr();
     check(fm_kv_read(&f, &r, stream), "fm_kv_read");
-    const Tensor q = rows(query), out = fresh({B, S, Hq, f.dv}, q.scalar_type(), ck), lse = fresh({B, Hq, S}, at::kFloat, ck);
+    const Tensor q = rows(vec_rows(query)), out = fresh({B, S, Hq, f.dv}, q.scalar_type(), ck), lse = fresh({B, Hq, S}, at::kFloat, ck);
     int tm = 0, tn = 0;
     check(fm_fwd_tile_shape(f.d, f.dv, &tm, &tn), "fm_fwd_tile_shape");
     const Tensor minmax = scan_mask(bounds, (int)S, causal, tm, tn, stream);
