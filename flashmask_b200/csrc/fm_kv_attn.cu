@@ -66,17 +66,6 @@ __device__ __forceinline__ uint32_t k_at(int r, int c) { return r * (DK * 64) + 
 template <int VC>
 __device__ __forceinline__ uint32_t v_at(int r, int c) { return r * (VC * 8) + ((VC == 8 ? c ^ (r >> 1 & 3) : c ^ ((r >> 1 & 3) << 1)) << 4); }
 
-__device__ __forceinline__ uint4 lds128(uint32_t at) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
-  return r;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t at) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
-  return r;
-}
-
 // What the rows of a sequence may see: rows i < n stand at p0 + i; keys [lo, hi) are seen by one of them at least.
 struct KvRange { int len, n, p0, lo, hi; };
 __device__ __forceinline__ KvRange kv_range(const KvAttnParams& p, int b) {
@@ -105,9 +94,15 @@ __device__ __forceinline__ void row_range(const KvAttnParams& p, const KvRange& 
   if (p.window > 0) lo = max(0, r.p0 + i + 1 - p.window);
 }
 
+// (not volatile, as the products: the compiler may order what does not depend on each other)
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 
@@ -423,7 +418,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
           for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
       }
     }
-    const uint32_t from = ring + stage * Cfg::STAGE;
+    const unsigned char* from = smem + (warp * STAGES + stage) * Cfg::STAGE;
     stage = stage + 1 == STAGES ? 0 : stage + 1;
     const int k0 = seg.key0 + KV_BLOCK * warp + (i - seg_end + seg.u1 - seg.u0) * KV_UNIT;
 
@@ -439,8 +434,8 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
       uint4 x[2][2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
-        x[hh][0] = lds128(from + hh * Cfg::GROUP + k_at<DK>(g, t + 4 * c));
-        x[hh][1] = lds128(from + hh * Cfg::GROUP + k_at<DK>(g + 8, t + 4 * c));
+        x[hh][0] = *reinterpret_cast<const uint4*>(from + hh * Cfg::GROUP + k_at<DK>(g, t + 4 * c));
+        x[hh][1] = *reinterpret_cast<const uint4*>(from + hh * Cfg::GROUP + k_at<DK>(g + 8, t + 4 * c));
       }
       const uint2* q = s_q + c * 128 + lane;
 #pragma unroll
@@ -457,7 +452,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
         for (int nt = 0; nt < NT; ++nt) {
           const uint2 y = q[nt * DK * 128 + j * 32];
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) mma16816<false>(s[nt][hh], fr[hh], y.x, y.y);
+          for (int hh = 0; hh < 2; ++hh) mma(s[nt][hh], fr[hh], y.x, y.y);
         }
       }
     }
@@ -533,14 +528,14 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int r = 2 * t + (x & 1) + (x >> 1) * 8;
-        const uint32_t at = from + hh * Cfg::GROUP + 16 * Cfg::KP;
+        const unsigned char* at = from + hh * Cfg::GROUP + 16 * Cfg::KP;
         if constexpr (VC == 8) {
-          const uint2 v = lds64(at + v_at<VC>(r, g >> 1) + (g & 1) * 8);
+          const uint2 v = *reinterpret_cast<const uint2*>(at + v_at<VC>(r, g >> 1) + (g & 1) * 8);
           vc[x][0] = v.x; vc[x][1] = v.y;
         } else {
 #pragma unroll
           for (int c = 0; c < VC / 16; ++c) {
-            const uint4 v = lds128(at + v_at<VC>(r, g + 8 * c));
+            const uint4 v = *reinterpret_cast<const uint4*>(at + v_at<VC>(r, g + 8 * c));
             vc[x][4 * c] = v.x; vc[x][4 * c + 1] = v.y; vc[x][4 * c + 2] = v.z; vc[x][4 * c + 3] = v.w;
           }
         }
@@ -575,7 +570,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
                 float w[4], seen[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) w[q] = hidden >> (nt * 8 + hh * 4 + q) & 1u ? 0.f : 1.f;
-                mma16816<false>(seen, fr, movmatrix_trans(pack2<false>(w[0], w[1])), movmatrix_trans(pack2<false>(w[2], w[3])));
+                mma(seen, fr, movmatrix_trans(pack2<false>(w[0], w[1])), movmatrix_trans(pack2<false>(w[2], w[3])));
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                   if (seen[q] > 0.f) o[nt][2 * c + half][q] = __uint_as_float(0x7fffffffu);
@@ -593,7 +588,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
           from_payload4<INT8>(__byte_perm(vc[0][c], vc[1][c], sel), fr[0], fr[1]);
           from_payload4<INT8>(__byte_perm(vc[2][c], vc[3][c], sel), fr[2], fr[3]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816<false>(o[nt][2 * c + half], fr, pb[0][nt][0], pb[0][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma(o[nt][2 * c + half], fr, pb[0][nt][0], pb[0][nt][1]);
         }
       }
 #pragma unroll
