@@ -30,7 +30,7 @@ __device__ __forceinline__ RowWalk row_walk(int upr) {
 // of the earlier tokens is rounded on the new grid.  Slots behind the last new token are left as they are.
 // VEC = units of 8 values that a thread holds.
 template <bool IS_BF16, bool INT8, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS, VEC <= 4 ? 1280 / THREADS : (VEC <= 8 ? 2 : 1)) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) : (VEC == 1 ? 1280 / THREADS : (VEC <= 8 ? 2 : 1))) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
   constexpr int WARPS = THREADS / 32;
   __shared__ uint32_t s_max[WARPS];
   const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, P = 1 << p.g.page_log2;
@@ -262,14 +262,17 @@ static unsigned pages_of(int S, int page_size) { return (unsigned)(((int64_t)S +
 template <bool IS_BF16, bool INT8>
 static int launch_write(const KvWriteParams& p, int page_size, int width_max, cudaStream_t s) {
   const dim3 grid(pages_of(p.S, page_size), 2 * p.g.Hkv, p.B);
-  const int upr = width_max / 8, rows = std::min(page_size, p.S), vec = (rows + 256 / upr - 1) / (256 / upr);      // <= 16
-  // (a few tokens: a CTA of 64 threads has a unit for each, and 2048 of them fit the chip at once)
-  if (rows <= 64 / upr) kv_write_kernel<IS_BF16, INT8, 1, 64><<<grid, 64, 0, s>>>(p);
-  else if (vec <= 1) kv_write_kernel<IS_BF16, INT8, 1, 256><<<grid, 256, 0, s>>>(p);
-  else if (vec <= 2) kv_write_kernel<IS_BF16, INT8, 2, 256><<<grid, 256, 0, s>>>(p);
-  else if (vec <= 4) kv_write_kernel<IS_BF16, INT8, 4, 256><<<grid, 256, 0, s>>>(p);
-  else if (vec <= 8) kv_write_kernel<IS_BF16, INT8, 8, 256><<<grid, 256, 0, s>>>(p);
-  else kv_write_kernel<IS_BF16, INT8, 16, 256><<<grid, 256, 0, s>>>(p);
+  const int upr = width_max / 8, rows = std::min(page_size, p.S);
+  auto holds = [&](int threads, int vec) { return rows <= threads / upr * vec; };
+  // A few tokens: a CTA of 64 threads has a unit for each, and 2048 of them fit the chip at once.  Whole pages: CTAs of 128
+  // threads, eight to an SM (64 tokens of 128 values, 2 x 8192 of them with 8 heads: 17 us, 5.9 TB/s; 256 threads of four units,
+  // five to an SM: 20 us; 512 threads of two: 29 us).
+  if (holds(64, 1)) kv_write_kernel<IS_BF16, INT8, 1, 64><<<grid, 64, 0, s>>>(p);
+  else if (holds(256, 1)) kv_write_kernel<IS_BF16, INT8, 1, 256><<<grid, 256, 0, s>>>(p);
+  else if (holds(128, 4)) kv_write_kernel<IS_BF16, INT8, 4, 128><<<grid, 128, 0, s>>>(p);
+  else if (holds(128, 8)) kv_write_kernel<IS_BF16, INT8, 8, 128><<<grid, 128, 0, s>>>(p);
+  else if (holds(256, 8)) kv_write_kernel<IS_BF16, INT8, 8, 256><<<grid, 256, 0, s>>>(p);
+  else kv_write_kernel<IS_BF16, INT8, 16, 256><<<grid, 256, 0, s>>>(p);       // (128 tokens of 256 values: 4096 units; any width: 240 threads hold them)
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   return FM_OK;
