@@ -142,7 +142,7 @@ struct KvReadParams {
 // Bound by HBM: 3 bytes a value.
 constexpr int READ_ILP = 4;
 template <bool IS_BF16, bool INT8>
-__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvReadParams p) {
+__global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__ KvReadParams p) {
   const int b = blockIdx.z, h = blockIdx.y, P = 1 << p.g.page_log2;
   const int64_t start = p.start[b], base = ((start >> p.g.page_log2) + blockIdx.x) << p.g.page_log2;      // (rounds down below 0 too)
   const int len = kv_len(p.g, p.seqlens[b]);
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
   const int lo = base < start ? (int)(start - base) : 0, hi = (int)min((int64_t)P, start + p.S - base);    // slots that are asked for
   const int valid = page >= 0 ? (int)min((int64_t)P, len - base) : 0;                                      // slots that hold tokens
   const size_t ph = (size_t)max(page, 0) * p.g.Hkv + h;
-  const RowWalk at[2] = {row_walk<256>(p.width[0] >> 3), row_walk<256>(p.width[1] >> 3)};
+  const RowWalk at[2] = {row_walk<128>(p.width[0] >> 3), row_walk<128>(p.width[1] >> 3)};
   float scale[2];
   const uint8_t* pay[2];
 #pragma unroll
@@ -327,8 +327,8 @@ extern "C" FM_API int fm_kv_read(const fm_kv_cache* c, const fm_kv_args* a, void
   const dim3 grid(pages_of(a->S, c->page_size), c->Hkv, a->B);
   const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
   cudaStream_t s = (cudaStream_t)stream;
-  if (bf) { if (i8) kv_read_kernel<true, true><<<grid, 256, 0, s>>>(p); else kv_read_kernel<true, false><<<grid, 256, 0, s>>>(p); }
-  else { if (i8) kv_read_kernel<false, true><<<grid, 256, 0, s>>>(p); else kv_read_kernel<false, false><<<grid, 256, 0, s>>>(p); }
+  if (bf) { if (i8) kv_read_kernel<true, true><<<grid, 128, 0, s>>>(p); else kv_read_kernel<true, false><<<grid, 128, 0, s>>>(p); }
+  else { if (i8) kv_read_kernel<false, true><<<grid, 128, 0, s>>>(p); else kv_read_kernel<false, false><<<grid, 128, 0, s>>>(p); }
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   return FM_OK;
