@@ -2,23 +2,29 @@
 //
 // All query rows of a kv head (queries x heads of its group) read the same keys, so they form one item's rows, eight to
 // a column tile of mma.m16n8k16: S^T = K Q^T with the keys as rows and O^T = V^T P^T with the values' dims as rows,
-// which fills the instruction from one row on (rows as M would fill a half or a quarter of it).  The payload goes from
-// HBM to registers in the order in which the fragments want it and is widened there: fp16 holds every payload value.
-//   K: lane (g, t) loads 16-byte chunks t, t + 4, .. of keys g and g + 8; four values of a chunk are one k-step's share
+// which fills the instruction from one row on (rows as M would fill a half or a quarter of it).  The payload is copied to a
+// ring in shared memory by its bytes, and a lane reads it in the order in which the fragments want it and widens it in
+// registers: fp16 holds every payload value.
+//   K: lane (g, t) reads 16-byte chunks t, t + 4, .. of keys g and g + 8; four values of a chunk are one k-step's share
 //      of the lane, and Q is laid out with the same permutation of the head dim.
-//   V: lane (g, t) loads chunk g of keys 2t, 2t + 1, 2t + 8, 2t + 9; byte pairs of two keys are the A operand's pairs
+//   V: lane (g, t) reads chunk g of keys 2t, 2t + 1, 2t + 8, 2t + 9; byte pairs of two keys are the A operand's pairs
 //      along the keys, and byte 2j, 2j + 1 of chunk g are rows g, g + 8 of O^T's tile j.
 //   P^T: the S^T fragment, rounded to fp16 and transposed in registers (movmatrix).
 // q in bf16 is brought to fp16 by a power of two per row; p is in (0, 2^15], where fp16 has three bits more than bf16.
 //
-// Scales.  A page's k scale multiplies the scores.  Its v scale joins the exponent: with x = s + log2(vs) the kernel
-// keeps m = max x and p' = 2^(x - m), so that p' V8 sums are in units of 2^m for every page, and the denominator takes
-// p' / vs.  Powers of two: both are exact.
+// Scales.  A page's k scale multiplies the scores.  Its v scale joins the exponent: with x = s + log2(vs) and m at the
+// largest x the kernel keeps p' = 2^(x - m), so that sums of p' V8 are in units of 2^m for every page, and the
+// denominator takes p' / vs.  Powers of two: both are exact.
 //
 // Work.  The units (4 warps x 32 keys) of all items are laid out end to end and dealt evenly to one wave of CTAs, each
 // a contiguous range: sequences of any lengths load the chip evenly, and nothing about the lengths is needed on the
-// host.  A CTA leaves a partial result (fp32 O, l, m) where its range cuts an item; kv_attn_merge_kernel joins them.
-// Bound by HBM: (d + dv) bytes a key.
+// host.  A warp's copies run on across items.  A CTA leaves a partial result (fp32 O, l, m) where its range cuts an item;
+// kv_attn_merge_kernel joins them.
+//
+// Bound by HBM, (d + dv) bytes a key, once a call is long: 8 x 32768 keys, 32 / 8 heads, d = 128, one token: 89 us, 6.0
+// TB/s; 8 x 8192: 31 us, 4.3 TB/s (of which 5 us until the first data are there, 4 us behind the last, and CTAs that end between 20 and
+// 27 us: memory serves them unevenly); 64 x 4096, d = 64: 52 us, 5.2 TB/s.  From 16 rows on the dependent instructions of too few warps
+// bind, 8 x 8192 with 16 rows 38 us and 32 rows 54 us: 255 registers leave two CTAs to an SM.
 #include <algorithm>
 
 #include "fm_kv_cache.cuh"

@@ -137,16 +137,17 @@ __device__ __forceinline__ NormJob norm_job(const NormParams& p, int which, int6
 }
 
 // Forward.  A warp has one job, and the rows of the next two groups are on their way while one is worked on: 2 x 8192 tokens,
-// 32 / 8 heads, d = 128, bf16 (335 MB) in 62 us, 5.4 TB/s; with the backward's stream through shared memory 70 us.
+// 32 / 8 heads, d = 128, bf16 (335 MB) in 61 us, 5.5 TB/s; with the backward's stream through shared memory 70 us.  80
+// registers: six CTAs of 128 threads to an SM; at 72 the spills cost more than the seventh brings (64 us).
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
-__global__ void __launch_bounds__(256, 3) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(128, 6) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
   const int lane = threadIdx.x & 31, s = lane % LPR, sub = lane / LPR;
   constexpr int HPG = 32 / LPR;
   const bool on = s * 16 < p.d;
   int lo, hi;
   slot_offsets<INTERLEAVED>(s, p.rot, lo, hi);
   const int64_t tokens = (int64_t)p.B * p.S, q_jobs = tokens * p.chunks[0];
-  int64_t job = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int which = job >= q_jobs;
   if (which) job -= q_jobs;
   if (job >= tokens * p.chunks[which]) return;
@@ -294,7 +295,7 @@ __device__ __forceinline__ void read_angles(f2 (&c)[4], f2 (&sn)[4], uint32_t at
 }
 
 // Backward.  Warps walk q's jobs and then k's with a stride of the grid and keep the sums of dw of their slots in registers.
-// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 90 us, 5.6 TB/s; with the next group's rows in registers 110 us.
+// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 89 us, 5.7 TB/s; with the next group's rows in registers 110 us.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
 __global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   using Stream = NormStream<LPR>;
@@ -406,8 +407,9 @@ __global__ void __launch_bounds__(256) norm_rotary_dw_kernel(const NormSumParams
 // ---------------------------------------------------------------------------
 int sm_count();
 
-// A warp takes all heads of a token where there are tokens enough to fill the chip with warps (cos, sin and the weights
-// are loaded once for them), and one group of heads where there are few.
+// A warp takes all heads of a token where there are tokens enough to give each of an SM's 24 resident warps one (cos, sin
+// and the weights are loaded once for them), and fewer where there are few.  6002 tokens, 16 / 4 heads, d = 96, forward: all heads
+// 15.3 us, two halves 18.8 us.
 static void norm_plan(const fm_norm_rotary_args* a, NormParams* p) {
   p->B = a->B; p->S = a->S; p->d = a->d;
   const int lpr = a->d <= 128 ? 8 : (a->d <= 256 ? 16 : 32), hpg = 32 / lpr;
@@ -477,7 +479,7 @@ static int norm_launch(const NormParams& p, bool back, cudaStream_t s) {
     kern<<<(unsigned)norm_bwd_grid(p), 256, smem, s>>>(p);
   } else {
     const int64_t jobs = (int64_t)p.B * p.S * ((int64_t)p.chunks[0] + p.chunks[1]);
-    norm_rotary_fwd_kernel<IS_BF16, IL, LPR><<<(unsigned)((jobs + 7) / 8), 256, 0, s>>>(p);
+    norm_rotary_fwd_kernel<IS_BF16, IL, LPR><<<(unsigned)((jobs + 3) / 4), 128, 0, s>>>(p);
   }
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
