@@ -85,12 +85,19 @@ __device__ __forceinline__ KvRange kv_range(const KvAttnParams& p, int b) {
 }
 __device__ __forceinline__ int kv_units(const KvRange& r) { return max(1, (r.hi - r.lo + KV_UNIT - 1) / KV_UNIT); }
 
-// The units are dealt to n CTAs, the first total % n of which get one more.
-__device__ __forceinline__ int kv_first_unit(int total, int n, int c) { return total / n * c + min(c, total % n); }
-__device__ __forceinline__ int kv_cta_of(int total, int n, int unit) {
-  const int q = total / n, r = total % n;
-  return unit < r * (q + 1) ? unit / (q + 1) : r + (unit - r * (q + 1)) / q;
-}
+// How the units are dealt.  Every item counts `extra` slots behind its units, for the time that loading its queries and
+// joining its sums takes: about a unit's, so that CTAs with many short sequences end when the others do (64 ragged
+// sequences, d = 64: CTAs ended between 37 and 58 us without).  None where every unit gets a CTA of its own.  The slots are dealt to n CTAs, the
+// first slots % n of which get one more.
+struct KvDeal {
+  int n, extra, slots;
+  __device__ __forceinline__ KvDeal(int n_cta, int units, int n_items) : n(min(n_cta, units)), extra(units > n_cta ? 1 : 0), slots(units + n_items * extra) {}
+  __device__ __forceinline__ int first_slot(int c) const { return slots / n * c + min(c, slots % n); }
+  __device__ __forceinline__ int cta_of(int slot) const {
+    const int q = slots / n, r = slots % n;
+    return slot < r * (q + 1) ? slot / (q + 1) : r + (slot - r * (q + 1)) / q;
+  }
+};
 
 // Keys [lo, hi) that query row i sees; a row that is none sees nothing.
 __device__ __forceinline__ void row_range(const KvAttnParams& p, const KvRange& r, int i, int& lo, int& hi) {
@@ -165,9 +172,20 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
     if (b1 == p.B && b0 < b1) s_pre[p.B] = at + mine;
     __syncthreads();
   }
-  const int total = s_pre[p.B], n_cta = min(p.n_cta, total);            // (never a CTA without a unit between two with one)
-  if (blockIdx.x >= n_cta) return;
-  const int u_begin = kv_first_unit(total, n_cta, blockIdx.x), n_units = total / n_cta + (blockIdx.x < total % n_cta ? 1 : 0);
+  const KvDeal deal(p.n_cta, s_pre[p.B], p.B * items);
+  if (blockIdx.x >= deal.n) return;
+  // units before a slot
+  auto units_before = [&](int slot) {
+    if (deal.extra == 0 || slot >= deal.slots) return min(slot, s_pre[p.B]);
+    int b = 0, hi = p.B;
+#pragma unroll 1
+    while (hi - b > 1) { const int mid = (b + hi) >> 1; if (s_pre[mid] + mid * items <= slot) b = mid; else hi = mid; }
+    const int units = (s_pre[b + 1] - s_pre[b]) / items, in_seq = slot - s_pre[b] - b * items, item = in_seq / (units + 1);
+    return s_pre[b] + item * units + min(in_seq - item * (units + 1), units);
+  };
+  const int edge = units_before(deal.first_slot(blockIdx.x + (lane & 1)));          // (both ends of the range at once)
+  const int u_begin = __shfl_sync(0xffffffffu, edge, 0), n_units = __shfl_sync(0xffffffffu, edge, 1) - u_begin;
+  if (n_units == 0) return;
 
   // The part of the item of unit u that this CTA has from u on.
   auto segment = [&](int u) {
@@ -625,10 +643,11 @@ __global__ void __launch_bounds__(128) kv_attn_merge_kernel(const __grid_constan
   for (int o = 16; o; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); }
   if (lane == 0) { s_sum[0][warp] = all; s_sum[1][warp] = before; }
   __syncthreads();
-  const int total = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3], n = min(p.n_cta, total);
+  const KvDeal deal(p.n_cta, s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3], p.B * items);
   before = s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3];
   const int tile = row / ROWS, in_tile = row - tile * ROWS;
-  const int s0 = before + (h * p.row_tiles + min(tile, p.row_tiles - 1)) * mine, c0 = kv_cta_of(total, n, s0), c1 = kv_cta_of(total, n, s0 + mine - 1);
+  const int s0 = before + b * items * deal.extra + (h * p.row_tiles + min(tile, p.row_tiles - 1)) * (mine + deal.extra);
+  const int c0 = deal.cta_of(s0), c1 = deal.cta_of(s0 + mine - 1);
   grid_dep_wait();
   if (c0 == c1 || row >= p.S * p.G) return;               // done by one CTA; no row
   auto slot = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * ROWS + in_tile; };
@@ -789,7 +808,7 @@ extern "C" FM_API int fm_kv_attention(const fm_kv_cache* c, const fm_kv_args* a,
   const KvAttnPlan pl = kv_attn_plan(c, a);
   const int64_t G = a->Hq / c->Hkv, rows = a->S * G, tiles = (rows + pl.nt * 8 - 1) / (pl.nt * 8);
   const int64_t units = ((int64_t)a->max_pages * c->page_size + 31) / KV_UNIT + 1;
-  FM_REQUIRE(rows < 1 << 30 && units * tiles <= (INT_MAX - 1) / c->Hkv / a->B, FM_ERR_UNSUPPORTED, "fm_kv_attention: too many rows and keys for one call");
+  FM_REQUIRE(rows < 1 << 30 && (units + 1) * tiles <= (INT_MAX - 1) / c->Hkv / a->B, FM_ERR_UNSUPPORTED, "fm_kv_attention: too many rows and keys for one call");
   FM_REQUIRE((int64_t)c->num_pages * c->Hkv * c->page_size / 16 < INT_MAX, FM_ERR_UNSUPPORTED, "fm_kv_attention: a cache of 2^31 groups of 16 tokens");
   FM_REQUIRE(a->workspace && a->workspace_bytes >= pl.bytes && ((uintptr_t)a->workspace & 15) == 0, FM_ERR_WORKSPACE,
              "fm_kv_attention: workspace of %zu bytes, %zu needed", a->workspace_bytes, pl.bytes);
