@@ -388,7 +388,13 @@ __global__ void __launch_bounds__(256) norm_rotary_dw_kernel(const NormSumParams
   __shared__ float s[32][9];
   float v = 0.f;
   if (j < 2 * p.d)
-    for (int i = k; i < p.n; i += 32) v += p.part[(size_t)i * 2 * p.d + j];
+    for (int i = k; i < p.n; i += 32 * 5) {                 // (five loads in flight: 296 CTAs' sums are two rounds)
+      float x[5];
+#pragma unroll
+      for (int a = 0; a < 5; ++a) x[a] = i + 32 * a < p.n ? __ldcg(p.part + (size_t)(i + 32 * a) * 2 * p.d + j) : 0.f;
+#pragma unroll
+      for (int a = 0; a < 5; ++a) v += x[a];
+    }
   s[k][threadIdx.x & 7] = v;
   __syncthreads();
   if (threadIdx.x >= 8 || j >= 2 * p.d) return;
