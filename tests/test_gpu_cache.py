@@ -467,6 +467,37 @@ def test_generation_replays_from_a_cuda_graph():
         assert torch.equal(getattr(cache, n).view(torch.uint8), getattr(cache2, n).view(torch.uint8))
 
 
+def test_two_graphs_and_two_streams_share_nothing():
+    """Two captured calls replayed in turn and against each other on two streams, one with many parts, one through the dense forward."""
+    f, g = Filled([3000, 900], 2, 128, 128, E4M3, 64, seed=25), Filled([700, 333], 2, 128, 128, INT8, 32, seed=26)
+    q1, q2 = rand_q(2, 1, 8, 128).cuda(), rand_q(2, 40, 8, 128, seed=2).cuda()
+    args = [(q1, f.cache, f.table.cuda(), f.seqlens.cuda()), (q2, g.cache, g.table.cuda(), g.seqlens.cuda())]
+    want = [fm.kv_cache_attention(*a, return_lse=True) for a in args]
+    graphs, got = [], []
+    for a in args:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(fm.kv_cache_attention(*a, return_lse=True))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x in got:
+            for t in x:
+                t.zero_()
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = []
+        for a, s in zip(args, streams):
+            with torch.cuda.stream(s):
+                eager.append(fm.kv_cache_attention(*a, return_lse=True))
+        torch.cuda.synchronize()
+        for w, x, y in zip(want, got, eager):
+            for a, b, c in zip(w, x, y):
+                assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_prompt_then_tokens_is_attention_over_everything():
     """A prompt written and attended to in one call, then token by token: every step against the dense operator over what
     the cache gives back, within the rounding of p and of the output."""

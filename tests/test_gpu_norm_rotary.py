@@ -202,6 +202,33 @@ def test_before_the_attention_of_a_training_step():
         assert (a.double() - b).norm() <= 8 * 2.0 ** -9 * b.norm(), ((a.double() - b).norm() / b.norm())
 
 
+def test_forward_and_gradients_replay_from_a_cuda_graph():
+    """Replays with new inputs give the bits of eager calls.  (No eager graph of the same leaves may live at the capture: torch ties a
+    leaf to the stream of its first graph.)"""
+    q, k, gq, gk, w, cos, sin, pos = problem(2, 300, 8, 2, 128, 64, torch.bfloat16, torch.float32, seed=11)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, *w)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = fm.qk_norm_rotary(*leaves, cos, sin, pos)
+        torch.autograd.grad(out, leaves, [gq, gk])
+        del out
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fm.qk_norm_rotary(*leaves, cos, sin, pos)
+        grads = torch.autograd.grad(out, leaves, [gq, gk])
+    for seed in (12, 13):
+        q2, k2, gq2, gk2, w2, _, _, pos2 = problem(2, 300, 8, 2, 128, 64, torch.bfloat16, torch.float32, seed=seed)
+        with torch.no_grad():
+            for a, b in zip((*leaves, gq, gk, pos), (q2, k2, *w2, gq2, gk2, pos2)):
+                a.copy_(b)
+        graph.replay()
+        want, wgrads = check(q2, k2, gq2, gk2, w2, cos, sin, pos2)
+        for a, b in zip((*out, *grads), (*want, *wgrads)):
+            assert torch.equal(a, b)
+
+
 def test_refusals():
     q, k, _, _, w, cos, sin, pos = problem(1, 4, 4, 2, 64, 32, torch.bfloat16, torch.float32, seed=9)
     ok = lambda q=q, k=k, w=w, cos=cos, sin=sin, pos=pos, **kw: fm.qk_norm_rotary(q, k, *w, cos, sin, pos, **kw)
