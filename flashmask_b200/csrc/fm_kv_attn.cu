@@ -123,7 +123,14 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // What a range of units of one item is: the item, and which of its keys.
-struct KvSegment { int b, h, row0, units, u0, u1, key0; KvRange r; };
+struct KvSegment {
+  int b, h, row0, units, u0, u1, key0;
+  KvRange r;
+  __device__ __forceinline__ KvSegment of_lane(int x) const {
+    auto s = [&](int v) { return __shfl_sync(0xffffffffu, v, x); };
+    return {s(b), s(h), s(row0), s(units), s(u0), s(u1), s(key0), {s(r.len), s(r.n), s(r.p0), s(r.lo), s(r.hi)}};
+  }
+};
 
 // FULL: d = 64 DK and dv = 8 VC, known to the compiler.
 // The loops over chunks of the head dim and over the two groups stay loops: short calls run every instruction once or
@@ -207,30 +214,36 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
 
   // Groups j = 2 i + (0, 1) of the warp's block in unit u_begin + i.  They are looked up 32 at a time, a lane each and across
   // items, and kept in shared memory: the index of the group in the cache (-1: none), which the copies need, and (ks,
-  // log2 vs, 1 / vs) behind the first copies.  A group that is none has scores of -inf and values of 0.
+  // log2 vs, 1 / vs) behind the first copies.  A group that is none has scores of -inf and values of 0.  In steps, between which
+  // the first round has other work to do: the page number is asked for, the place stored, the scales asked for, and stored.
   float4* info = s_info + warp * KV_INFO;
-  int page = -1, head = 0;
-  auto look_up_place = [&](int first) {
+  KvSegment ahead = {};
+  int number = -1, page = -1, key = 0;
+  float ks = 0.f, vs = 1.f;
+  auto ask_page = [&](int first) {
     const int i = (first + lane) >> 1;
-    int at = -1;
-    page = -1;
+    number = -1;
     if (i < n_units) {
-      const KvSegment s = segment(u_begin + i);
-      const int key = s.key0 + KV_BLOCK * warp + (lane & 1) * 16;
-      head = s.h;
-      if (key < s.r.hi) page = kv_page(p.g, p.table + s.b * p.g.table_stride, key);
-      if (page >= 0) at = ((page * p.g.Hkv + head) << (p.g.page_log2 - 4)) + ((key & ((1 << p.g.page_log2) - 1)) >> 4);
+      ahead = segment(u_begin + i);
+      key = ahead.key0 + KV_BLOCK * warp + (lane & 1) * 16;
+      if (key < ahead.r.hi) number = kv_page_number(p.g, p.table + ahead.b * p.g.table_stride, key);
     }
+  };
+  auto store_place = [&](int first) {
+    page = kv_page_in(p.g, number);
+    const int at = page < 0 ? -1 : ((page * p.g.Hkv + ahead.h) << (p.g.page_log2 - 4)) + ((key & ((1 << p.g.page_log2) - 1)) >> 4);
     info[(first + lane) & (KV_INFO - 1)].w = __int_as_float(at);
     __syncwarp();
   };
-  auto look_up_scale = [&](int first) {
-    float ks = 0.f, vs = 1.f;
+  auto ask_scale = [&]() {
+    ks = 0.f; vs = 1.f;
     if (page >= 0) {
-      const int64_t ph = (int64_t)page * p.g.Hkv + head;
+      const int64_t ph = (int64_t)page * p.g.Hkv + ahead.h;
       ks = __ldg(p.ks + ph);
       vs = __ldg(p.vs + ph);
     }
+  };
+  auto store_scale = [&](int first) {
     float4* to = &info[(first + lane) & (KV_INFO - 1)];
     to->x = ks;
     to->y = page >= 0 ? log2f(vs) : -INFINITY;
@@ -241,7 +254,10 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
   // The copies of the warp's block in unit i, 16 bytes a lane; zeros behind the head dim.  One commit for every call.
   auto fetch = [&](int i, int stage) {
     if (i < n_units) {
-      if ((i & 15) == 0) look_up_place(2 * i);
+      if ((i & 15) == 0) {
+        if (i > 0) ask_page(2 * i);
+        store_place(2 * i);
+      }
 #pragma unroll 1
       for (int hh = 0; hh < 2; ++hh) {
         const int at = __float_as_int(info[(2 * i + hh) & (KV_INFO - 1)].w);
@@ -260,10 +276,15 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
           cp_async16(to + 16 * Cfg::KP + v_at<VC>(r, c), vp + (FULL || on ? r * dv + c * 16 : 0), on);
         }
       }
-      if ((i & 15) == 0) look_up_scale(2 * i);
+      if ((i & 15) == 0) {
+        ask_scale();
+        if (NT > 3 || i > 0) store_scale(2 * i);         // (32 rows leave no registers for it to wait in)
+      }
     }
     cp_async_commit();
   };
+
+  ask_page(0);
 
   float f[NT][2], m[NT][2], l[NT][2], o[NT][MT][4];      // of the lane's columns 2t, 2t + 1
 
@@ -351,20 +372,22 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
   };
 
   KvSegment seg;
-  int seg_end = 0, lo_max = 0, hi_min = 0, stage = 0, free_stage = 0;
+  int seg_end = INT_MIN, lo_max = 0, hi_min = 0, stage = 0, free_stage = 0;
 #pragma unroll 1
   for (int i = 1 - STAGES; i <= n_units; ++i) {
     if (i >= 0 && i < n_units) {
       cp_async_wait<STAGES - 2>();
       __syncwarp();                                    // block i is here, and every lane is done with block i - 1
     }
-    const bool turn = i == seg_end;
+    // (the first item's turn comes ahead of its data)
+    const bool turn = i == seg_end || i == 1 - STAGES;
     KvSegment last;
     uint4 x[DK][2];
     if (turn) {
       // the next item's queries (row g of tile `warp`) are on their way while the last one's sums are joined
       last = seg;
-      if (i < n_units) seg = segment(u_begin + i);
+      if (i < 0) seg = ahead.of_lane(0);
+      else if (i < n_units) seg = segment(u_begin + i);
       const int row = seg.row0 + warp * 8 + g, qi = row / p.G;
       const bool on = warp < NT && i < n_units && qi < p.S;
       const uint16_t* src = p.q + seg.b * p.qs[0] + qi * p.qs[1] + ((int64_t)seg.h * p.G + row - qi * p.G) * p.qs[2];
@@ -382,9 +405,8 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
     }
     fetch(i + STAGES - 1, free_stage);
     free_stage = free_stage + 1 == STAGES ? 0 : free_stage + 1;
-    if (i < 0) continue;
     if (turn) {
-      seg_end = i + seg.u1 - seg.u0;
+      seg_end = max(i, 0) + seg.u1 - seg.u0;
       if (tid < ROWS) {
         const int row = (seg.row0 + tid) / p.G;
         int lo, hi;
@@ -427,6 +449,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
         }
         if (t == 0) s_f[warp * 8 + g] = scale * p.scale_log2;
       }
+      if (NT <= 3 && i < 0) store_scale(0);
       __syncthreads();                                    // s_lim, s_q, s_f
       lo_max = 0; hi_min = INT_MAX;
       if (lane < ROWS) { lo_max = s_lim[lane].x; hi_min = s_lim[lane].y; }
@@ -442,6 +465,7 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
           for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.f;
       }
     }
+    if (i < 0) continue;
     const unsigned char* from = smem + (warp * STAGES + stage) * Cfg::STAGE;
     stage = stage + 1 == STAGES ? 0 : stage + 1;
     const int k0 = seg.key0 + KV_BLOCK * warp + (i - seg_end + seg.u1 - seg.u0) * KV_UNIT;

@@ -22,14 +22,13 @@ struct KvGeom {
 
 // Page of position `pos` of the sequence whose page table row is `row`, or -1: the position is outside of the table, or
 // the table names no page of the cache.  The only place where a page number is turned into something to address with;
-// fm_kv_locate runs it on the host.
-__host__ __device__ __forceinline__ int kv_page(const KvGeom& g, const int32_t* row, int pos) {
-  if (pos < 0) return -1;
+// fm_kv_locate runs it on the host.  In two steps for who has other work while the table is read.
+__host__ __device__ __forceinline__ int kv_page_number(const KvGeom& g, const int32_t* row, int pos) {
   const int j = pos >> g.page_log2;
-  if (j >= g.max_pages) return -1;
-  const int page = row[j];
-  return page >= 0 && page < g.num_pages ? page : -1;
+  return pos < 0 || j >= g.max_pages ? -1 : row[j];
 }
+__host__ __device__ __forceinline__ int kv_page_in(const KvGeom& g, int page) { return page >= 0 && page < g.num_pages ? page : -1; }
+__host__ __device__ __forceinline__ int kv_page(const KvGeom& g, const int32_t* row, int pos) { return kv_page_in(g, kv_page_number(g, row, pos)); }
 
 // Length of a sequence as the kernels use it: never beyond its page table.
 __host__ __device__ __forceinline__ int kv_len(const KvGeom& g, int len) { return len < 0 ? 0 : (len > g.cap ? g.cap : len); }
