@@ -7,7 +7,7 @@
 // Bound by HBM: 4 bytes a value forward (x in, y out), 6 backward (x and dy in, dx out); nothing is kept between the
 // two, since r costs no memory once x has to be read again.  A row of d values is d / 16 slots of 16: two vectors of 8
 // that hold both halves of 8 pairs (or, with neighbouring pairs, and behind the rotated part, 16 values in a row), so a
-// thread turns its own pairs and the only exchange is the row's sum, over 8, 16 or 32 lanes.  The heads of a token share its
+// thread turns its own pairs and the only exchange is the row's sum, over 4, 8, 16 or 32 lanes.  The heads of a token share its
 // cos and sin: a warp stays with one token and walks its heads.
 #include <algorithm>
 
@@ -15,6 +15,19 @@
 #include "fm_kv_cache.cuh"
 
 namespace fm {
+
+// n / d for 0 <= n < 2^31 by a product: m = floor(2^(31 + l) / d) + 1 with 2^l >= d is too large by at most d / 2^(31 + l) of 1, which
+// times n stays below 1 / d.  A job's place takes two divisions, and many jobs are two groups of rows.
+struct Div {
+  uint32_t m; int shift;
+  void set(int d) {
+    int l = 0;
+    while ((int64_t)1 << l < d) ++l;
+    shift = 31 + l;
+    m = d > 0 ? (uint32_t)(((uint64_t)1 << shift) / d + 1) : 0;
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t)(uint32_t)n * m >> shift); }
+};
 
 struct NormParams {
   const uint16_t* x[2]; uint16_t* y[2];                        // q, k: inputs; outputs (backward: dx)
@@ -26,6 +39,7 @@ struct NormParams {
   const void* pos; int pos64; int64_t pos_b;                   // [B, S] with that batch stride, or NULL: the token's index
   int B, S, H[2], d, rot, table, w_f32;
   int chunks[2], per_chunk[2];                                 // a token's groups of 32 / LPR heads are dealt to `chunks` jobs
+  Div by_S, by_chunks[2];
   float eps, inv_d;
 };
 
@@ -126,18 +140,13 @@ __device__ __forceinline__ void load_angles(const NormParams& p, int64_t b, int 
 
 // A warp's job: a token of q or of k and `per_chunk` of its groups of 32 / LPR heads.  All of q's jobs come before k's.
 struct NormJob { int64_t b; int t, g0, g1; };
-__device__ __forceinline__ NormJob norm_job(const NormParams& p, int which, int64_t job, int groups) {
-  NormJob j;
-  const int64_t token = job / p.chunks[which];
-  j.b = token / p.S;
-  j.t = (int)(token - j.b * p.S);
-  j.g0 = (int)(job - token * p.chunks[which]) * p.per_chunk[which];
-  j.g1 = min(j.g0 + p.per_chunk[which], groups);
-  return j;
+__device__ __forceinline__ NormJob norm_job(const NormParams& p, int which, int job, int groups) {
+  const int token = p.by_chunks[which](job), b = p.by_S(token), g0 = (job - token * p.chunks[which]) * p.per_chunk[which];
+  return {b, token - b * p.S, g0, min(g0 + p.per_chunk[which], groups)};
 }
 
 // Forward.  A warp has one job, and the rows of the next two groups are on their way while one is worked on: 2 x 8192 tokens,
-// 32 / 8 heads, d = 128, bf16 (335 MB) in 61 us, 5.5 TB/s; with the backward's stream through shared memory 70 us.  80
+// 32 / 8 heads, d = 128, bf16 (335 MB) in 59 us, 5.7 TB/s; with the backward's stream through shared memory 70 us.  80
 // registers: six CTAs of 128 threads to an SM; at 72 the spills cost more than the seventh brings (64 us).
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
 __global__ void __launch_bounds__(128, 6) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
@@ -146,8 +155,8 @@ __global__ void __launch_bounds__(128, 6) norm_rotary_fwd_kernel(const __grid_co
   const bool on = s * 16 < p.d;
   int lo, hi;
   slot_offsets<INTERLEAVED>(s, p.rot, lo, hi);
-  const int64_t tokens = (int64_t)p.B * p.S, q_jobs = tokens * p.chunks[0];
-  int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int tokens = p.B * p.S, q_jobs = tokens * p.chunks[0];
+  int job = blockIdx.x * 4 + (threadIdx.x >> 5);
   const int which = job >= q_jobs;
   if (which) job -= q_jobs;
   if (job >= tokens * p.chunks[which]) return;
@@ -191,57 +200,53 @@ __global__ void __launch_bounds__(128, 6) norm_rotary_fwd_kernel(const __grid_co
 }
 
 // A warp's stream of groups of rows: jobs `first`, `first` + `step`, .. of q or of k, a job being a token and some of its groups of
-// HPG = 32 / LPR heads.  Rows of x and dy are copied to shared memory DEPTH groups ahead, across jobs: a
-// lane copies what it will read itself, so nothing has to be waited for but the copies; and the angles of a job's token go to a ring
+// HPG = 32 / LPR heads.  Rows of x and dy are copied to shared memory DEPTH groups ahead, across jobs, a row's LPR lanes
+// copying its chunks of 16 bytes side by side whatever order they are read in (slots of 32 bytes, a chunk of each at a time, ask L2 for
+// every sector twice: neighbouring pairs 140 us instead of 91).  The angles of a job's token go to a ring
 // of their own, copied by one row's lanes for all.  (A group read in this step, DEPTH ahead of it, and the angles of the job behind:
 // DEPTH + 2 entries where every job is one group.)
-constexpr int NORM_DEPTH = 4;
+// CTAs of 256 threads are resident on an SM as registers (128) and shared memory allow: two, with rows of 32 lanes one, and
+// with rows of 16 lanes two at a depth of three (8192 tokens, 16 / 2 heads, d = 256: 50 us; one CTA at a depth of four 66 us).
+constexpr int norm_bwd_ctas(int lanes_per_row) { return lanes_per_row == 32 ? 1 : 2; }
 template <int LPR>
 struct NormStream {
+  static constexpr int DEPTH = LPR == 16 ? 3 : 4;
   static constexpr int HPG = 32 / LPR;
-  static constexpr int STAGE = 4 * 512, ANGLES = LPR * 64, BYTES = NORM_DEPTH * STAGE + (NORM_DEPTH + 2) * ANGLES;    // of a warp
+  static constexpr int STAGE = 4 * 512, ANGLES = LPR * 64, BYTES = DEPTH * STAGE + (DEPTH + 2) * ANGLES;    // of a warp
   const NormParams& p;
-  const int which, lane, s, sub, lo, hi, H, groups;
-  const bool on;
+  const int which, lane, s, sub, H, groups;
   const uint32_t ring, angles;
   const int jobs, step;
   // the copies' side
   int job, next_pos, g, g1, stage, entry;
   const uint16_t *x, *dy;
 
-  __device__ __forceinline__ NormStream(const NormParams& p_, int which_, uint32_t smem, int first, int step_, int lo_, int hi_)
-      : p(p_), which(which_), lane(threadIdx.x & 31), s(lane % LPR), sub(lane / LPR), lo(lo_), hi(hi_), H(p_.H[which_]),
-        groups((p_.H[which_] + HPG - 1) / HPG), on(s * 16 < p_.d), ring(smem), angles(smem + NORM_DEPTH * STAGE),
+  __device__ __forceinline__ NormStream(const NormParams& p_, int which_, uint32_t smem, int first, int step_)
+      : p(p_), which(which_), lane(threadIdx.x & 31), s(lane % LPR), sub(lane / LPR), H(p_.H[which_]),
+        groups((p_.H[which_] + HPG - 1) / HPG), ring(smem), angles(smem + DEPTH * STAGE),
         jobs(p_.B * p_.S * p_.chunks[which_]), step(step_), job(first), g(0), g1(0), stage(0), entry(0) {
     next_pos = position(job);
     begin();
   }
-  __device__ __forceinline__ void place(int j, int64_t& b, int& t, int& g0, int& g1_) const {
-    const int token = p.chunks[which] == 1 ? j : j / p.chunks[which], seq = token / p.S;
-    b = seq;
-    t = token - seq * p.S;
-    g0 = (j - token * p.chunks[which]) * p.per_chunk[which];
-    g1_ = min(g0 + p.per_chunk[which], groups);
-  }
+  __device__ __forceinline__ NormJob place(int j) const { return norm_job(p, which, j, groups); }
   // the position of job j's token, or -1: not in the tables
   __device__ __forceinline__ int position(int j) const {
     if (j >= jobs) return 0;
-    int64_t b; int t, g0, e;
-    place(j, b, t, g0, e);
-    if (!p.pos) return t;
-    const int64_t pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[b * p.pos_b + t] : reinterpret_cast<const int32_t*>(p.pos)[b * p.pos_b + t];
+    const NormJob a = place(j);
+    if (!p.pos) return a.t;
+    const int64_t pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[a.b * p.pos_b + a.t] : reinterpret_cast<const int32_t*>(p.pos)[a.b * p.pos_b + a.t];
     return pos >= 0 && pos < p.table ? (int)pos : -1;
   }
   // The job's rows from its first group on, and its angles: NaN where the tables do not have the position, so that the
   // mistake shows in the result.
   __device__ __forceinline__ void begin() {
     if (job >= jobs) return;
-    int64_t b; int t, g0;
-    place(job, b, t, g0, g1);
-    g = g0;
-    const int h = g0 * HPG + sub;
-    x = p.x[which] + b * p.xs[which][0] + t * p.xs[which][1] + h * p.xs[which][2];
-    dy = p.dy[which] + b * p.dys[which][0] + t * p.dys[which][1] + h * p.dys[which][2];
+    const NormJob a = place(job);
+    g = a.g0;
+    g1 = a.g1;
+    const int h = g * HPG + sub;
+    x = p.x[which] + a.b * p.xs[which][0] + a.t * p.xs[which][1] + h * p.xs[which][2];
+    dy = p.dy[which] + a.b * p.dys[which][0] + a.t * p.dys[which][1] + h * p.dys[which][2];
     const int pos = next_pos;
     next_pos = position(job + step);
     if (sub == 0) {
@@ -259,22 +264,29 @@ struct NormStream {
         for (int i = 0; i < 4; ++i) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(to + LPR * 16 * i), "r"(i < 2 ? c : n) : "memory");
       }
     }
-    entry = entry == NORM_DEPTH + 1 ? 0 : entry + 1;
+    entry = entry == DEPTH + 1 ? 0 : entry + 1;
   }
+  // Where chunk c of the lane's row is in a stage: the lanes of a row read neighbouring chunks or every second one, and eight
+  // that are served together then hit different banks.
+  __device__ __forceinline__ uint32_t chunk_at(int c) const { return (c >= LPR ? 512 : 0) + (sub * LPR + ((c ^ (c >> 3 & 1)) & (LPR - 1))) * 16; }
   // The copies of the next group; one commit for every call.
   __device__ __forceinline__ void fetch() {
     if (job < jobs) {
-      const bool live = on && g * HPG + sub < H;
-      const uint32_t to = ring + stage * STAGE + lane * 16;
-      cp_async16(to, live ? x + lo : p.x[which], live);
-      cp_async16(to + 512, live ? x + hi : p.x[which], live);
+      const bool row = g * HPG + sub < H;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = s + i * LPR;
+        const uint32_t to = ring + stage * STAGE + chunk_at(c);
+        if (row && c * 8 < p.d) {                                  // (what is not copied nobody uses)
+          cp_async16(to, x + c * 8, true);
+          cp_async16(to + 1024, dy + c * 8, true);
+        }
+      }
       x += HPG * p.xs[which][2];
-      cp_async16(to + 1024, live ? dy + lo : p.dy[which], live);
-      cp_async16(to + 1536, live ? dy + hi : p.dy[which], live);
       dy += HPG * p.dys[which][2];
       if (++g == g1) { job += step; begin(); }
     }
-    stage = stage + 1 == NORM_DEPTH ? 0 : stage + 1;
+    stage = stage + 1 == DEPTH ? 0 : stage + 1;
     cp_async_commit();
   }
 };
@@ -295,9 +307,9 @@ __device__ __forceinline__ void read_angles(f2 (&c)[4], f2 (&sn)[4], uint32_t at
 }
 
 // Backward.  Warps walk q's jobs and then k's with a stride of the grid and keep the sums of dw of their slots in registers.
-// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 89 us, 5.7 TB/s; with the next group's rows in registers 110 us.
+// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 82 us, 6.1 TB/s (4 x 4096, 16 / 4 heads, d = 64, 126 MB: 34 us); with the next group's rows in registers 110 us.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
-__global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(256, norm_bwd_ctas(LPR)) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   using Stream = NormStream<LPR>;
   constexpr int HPG = Stream::HPG;
   extern __shared__ __align__(128) unsigned char smem[];         // [8 warps] rings, sums [8][2][LPR * 16]
@@ -309,11 +321,12 @@ __global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_co
   if (p.part) grid_dep_trigger();                                // (the sum over the CTAs follows, and waits for this kernel's end)
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
-    const int step = gridDim.x * 8;
+    const int step = gridDim.x * 8, w0 = blockIdx.x * 8 + warp, first = which ? step - 1 - w0 : w0;      // (who had a job more of q's has one less of k's)
     __syncwarp();
-    Stream in(p, which, smem_u32(smem) + warp * Stream::BYTES, blockIdx.x * 8 + warp, step, lo, hi);
+    Stream in(p, which, smem_u32(smem) + warp * Stream::BYTES, first, step);
+    const uint32_t at_lo = in.chunk_at(lo >> 3), at_hi = in.chunk_at(hi >> 3);
 #pragma unroll 1
-    for (int i = 0; i < NORM_DEPTH; ++i) in.fetch();
+    for (int i = 0; i < Stream::DEPTH; ++i) in.fetch();
     f2 w[8], dw[8];
     if (on) load_weight<IS_BF16>(w, p.w[which], p.w_f32, lo, hi);
 #pragma unroll
@@ -321,39 +334,40 @@ __global__ void __launch_bounds__(256, 2) norm_rotary_bwd_kernel(const __grid_co
     int stage = 0, entry = 0;
     const int64_t yh = p.ys[which][2] * HPG;
 #pragma unroll 1
-    for (int job = blockIdx.x * 8 + warp; job < in.jobs; job += step) {
-      int64_t b; int t, g, g1;
-      in.place(job, b, t, g, g1);
-      uint16_t* y = p.y[which] + b * p.ys[which][0] + t * p.ys[which][1] + (int64_t)(g * HPG + sub) * p.ys[which][2];
+    for (int job = first; job < in.jobs; job += step) {
+      const NormJob a = in.place(job);
+      uint16_t* y = p.y[which] + a.b * p.ys[which][0] + a.t * p.ys[which][1] + (int64_t)(a.g0 * HPG + sub) * p.ys[which][2];
 #pragma unroll 1
-      for (; g < g1; ++g) {
-        cp_async_wait<NORM_DEPTH - 1>();
-        __syncwarp();                                            // the angles were copied by other lanes
-        const uint32_t from = in.ring + stage * Stream::STAGE + lane * 16;
-        stage = stage + 1 == NORM_DEPTH ? 0 : stage + 1;
+      for (int g = a.g0; g < a.g1; ++g) {
+        cp_async_wait<Stream::DEPTH - 1>();
+        __syncwarp();                                            // (other lanes' copies)
+        const uint32_t from = in.ring + stage * Stream::STAGE;
+        stage = stage + 1 == Stream::DEPTH ? 0 : stage + 1;
         f2 v[8], d[8], c[4], sn[4];
-        widen<IS_BF16>(v, Raw{lds_vec(from), lds_vec(from + 512)});
-        widen<IS_BF16>(d, Raw{lds_vec(from + 1024), lds_vec(from + 1536)});
+        widen<IS_BF16>(v, Raw{lds_vec(from + at_lo), lds_vec(from + at_hi)});
+        widen<IS_BF16>(d, Raw{lds_vec(from + 1024 + at_lo), lds_vec(from + 1024 + at_hi)});
         read_angles<LPR>(c, sn, in.angles + entry * Stream::ANGLES + s * 16);
+        __syncwarp();                                            // every lane has read the stage that is filled now
         in.fetch();
         const bool live = on && g * HPG + sub < in.H;
         turn<INTERLEAVED, true>(d, c, sn);
         f2 ss = mul(v[0], v[0]), dot = mul(mul(d[0], w[0]), v[0]);
 #pragma unroll
         for (int i = 1; i < 8; ++i) { ss = fma(v[i], v[i], ss); dot = fma(mul(d[i], w[i]), v[i], dot); }
-        const float r = 1.f / sqrtf(row_sum<LPR>(sum(ss)) * p.inv_d + p.eps), m = row_sum<LPR>(live ? sum(dot) : 0.f) * r * p.inv_d;
+        const float r = 1.f / sqrtf(row_sum<LPR>(live ? sum(ss) : 0.f) * p.inv_d + p.eps), m = row_sum<LPR>(live ? sum(dot) : 0.f) * r * p.inv_d;
         if (live) {
+          const float n = -r * r * m;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const f2 xr = mul(v[i], pair(r, r));
-            dw[i] = fma(d[i], xr, dw[i]);
-            v[i] = mul(fma(xr, pair(-m, -m), mul(d[i], w[i])), pair(r, r));
+            d[i] = mul(d[i], pair(r, r));
+            dw[i] = fma(d[i], v[i], dw[i]);
+            v[i] = fma(v[i], pair(n, n), mul(d[i], w[i]));
           }
           store<IS_BF16>(y, lo, hi, v);
         }
         y += yh;
       }
-      entry = entry == NORM_DEPTH + 1 ? 0 : entry + 1;
+      entry = entry == Stream::DEPTH + 1 ? 0 : entry + 1;
     }
     cp_async_wait<0>();
     // the warp's rows side by side; the warps below, in a fixed order
@@ -413,12 +427,15 @@ __global__ void __launch_bounds__(256) norm_rotary_dw_kernel(const NormSumParams
 // ---------------------------------------------------------------------------
 int sm_count();
 
+static int norm_lanes(int d) { return d <= 64 ? 4 : (d <= 128 ? 8 : (d <= 256 ? 16 : 32)); }       // of a row: LPR
+
 // A warp takes all heads of a token where there are tokens enough to give each of an SM's 24 resident warps one (cos, sin
 // and the weights are loaded once for them), and fewer where there are few.  6002 tokens, 16 / 4 heads, d = 96, forward: all heads
-// 15.3 us, two halves 18.8 us.
+// 15.3 us, two halves 18.8 us.  The backward has fewer warps, which walk the jobs; finer jobs, that would even out 3.5 tokens a warp,
+// bring nothing (8192 tokens, 32 / 8 heads, d = 128: 51 us either way).
 static void norm_plan(const fm_norm_rotary_args* a, NormParams* p) {
   p->B = a->B; p->S = a->S; p->d = a->d;
-  const int lpr = a->d <= 128 ? 8 : (a->d <= 256 ? 16 : 32), hpg = 32 / lpr;
+  const int hpg = 32 / norm_lanes(a->d);
   const int64_t tokens = (int64_t)a->B * a->S, warps = (int64_t)sm_count() * 24;
   const int64_t want = tokens > 0 ? (warps + tokens - 1) / tokens : 1;
   for (int i = 0; i < 2; ++i) {
@@ -426,7 +443,9 @@ static void norm_plan(const fm_norm_rotary_args* a, NormParams* p) {
     const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(want, groups));
     p->per_chunk[i] = (int)std::max<int64_t>(1, (groups + chunks - 1) / chunks);
     p->chunks[i] = (groups + p->per_chunk[i] - 1) / p->per_chunk[i];
+    p->by_chunks[i].set(p->chunks[i]);
   }
+  p->by_S.set(a->S);
 }
 
 static int norm_params(const fm_norm_rotary_args* a, bool back, NormParams* p) {
@@ -469,9 +488,8 @@ static int norm_params(const fm_norm_rotary_args* a, bool back, NormParams* p) {
   return FM_OK;
 }
 
-// Two CTAs of the backward per SM, as its registers allow.
 static int64_t norm_bwd_grid(const NormParams& p) {
-  const int64_t jobs = (int64_t)p.B * p.S * std::max(p.chunks[0], p.chunks[1]), most = (int64_t)sm_count() * 2;
+  const int64_t jobs = (int64_t)p.B * p.S * std::max(p.chunks[0], p.chunks[1]), most = (int64_t)sm_count() * norm_bwd_ctas(norm_lanes(p.d));
   return std::max<int64_t>(1, std::min((jobs + 7) / 8, most));
 }
 
@@ -493,7 +511,8 @@ static int norm_launch(const NormParams& p, bool back, cudaStream_t s) {
 }
 
 static int norm_dispatch(const NormParams& p, const fm_norm_rotary_args* a, bool back, cudaStream_t s) {
-#define FM_NORM(BF, IL) (p.d <= 128 ? norm_launch<BF, IL, 8>(p, back, s) : p.d <= 256 ? norm_launch<BF, IL, 16>(p, back, s) : norm_launch<BF, IL, 32>(p, back, s))
+  const int lpr = norm_lanes(p.d);
+#define FM_NORM(BF, IL) (lpr == 4 ? norm_launch<BF, IL, 4>(p, back, s) : lpr == 8 ? norm_launch<BF, IL, 8>(p, back, s) : lpr == 16 ? norm_launch<BF, IL, 16>(p, back, s) : norm_launch<BF, IL, 32>(p, back, s))
   if (a->dtype == FM_DTYPE_BF16) return a->interleaved ? FM_NORM(true, true) : FM_NORM(true, false);
   return a->interleaved ? FM_NORM(false, true) : FM_NORM(false, false);
 #undef FM_NORM

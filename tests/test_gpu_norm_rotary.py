@@ -249,3 +249,15 @@ def test_refusals():
         ok(cos=cos[:2], sin=sin[:2], pos=None)
     with pytest.raises(ValueError):
         ok(eps=-1.0)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,n", [(48, 16), (64, 32), (112, 56), (128, 32), (192, 96), (256, 128), (320, 64), (512, 256)])
+def test_several_tokens_a_warp(interleaved, d, n):
+    """Rows of every number of lanes, full ones and not, and heads that fill no group; what a kernel before left in shared memory
+    (here NaN) is no part of a row."""
+    full = 64 if d <= 64 else 128 if d <= 128 else 256 if d <= 256 else 512
+    bad = problem(1, 700, 9, 3, full, full // 2, torch.bfloat16, torch.float32, seed=7)
+    leaves = [torch.full_like(t, float("nan")).requires_grad_(True) for t in bad[:2]]
+    torch.autograd.grad(fm.qk_norm_rotary(*leaves, *bad[4], *bad[5:]), leaves, bad[2:4])
+    check(*problem(3, 1500, 9, 3, d, n, torch.bfloat16, torch.float32, seed=8), interleaved=interleaved)
