@@ -36,8 +36,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) 
   const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, P = 1 << p.g.page_log2;
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int start = p.start[b];
-  const int skip = start < 0 ? -start : 0;                       // rows before position 0 are not written
-  if (n <= skip || start > INT_MAX - p.S) return;
+  if (n + min(start, 0) <= 0 || start > INT_MAX - p.S) return;  // (rows before position 0 are not written)
   const int first = max(start, 0), last = start + n - 1;         // positions
   const int base = ((first >> p.g.page_log2) + (int)blockIdx.x) << p.g.page_log2;
   if (base > last || base < 0) return;
