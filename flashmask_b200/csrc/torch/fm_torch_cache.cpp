@@ -83,6 +83,20 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor& q_in, const Tensor& k_in, c
   return {qo, ko};
 }
 
+// A gradient that itself has none: with create_graph it is part of a graph that says so, and not a constant.
+class FirstOrder : public torch::autograd::Function<FirstOrder> {
+ public:
+  static Variable forward(AutogradContext*, const Variable& grad, const Variable&) { return grad.view_as(grad); }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "the gradients of qk_norm_rotary have no gradient");
+    return {};
+  }
+};
+Tensor first_order(const Tensor& grad) {
+  if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
+  return FirstOrder::apply(grad, at::empty({0}, grad.options()).requires_grad_(true));
+}
+
 class NormRotary : public torch::autograd::Function<NormRotary> {
  public:
   static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k, const std::optional<Tensor>& qw_in,
@@ -116,7 +130,7 @@ class NormRotary : public torch::autograd::Function<NormRotary> {
       a.workspace = ws.data_ptr();
     }
     check(fm_norm_rotary_bwd(&a, stream_of(q)), "fm_norm_rotary_bwd");
-    return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {first_order(dq), first_order(dk), first_order(dqw), first_order(dkw), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 

@@ -261,3 +261,15 @@ def test_several_tokens_a_warp(interleaved, d, n):
     leaves = [torch.full_like(t, float("nan")).requires_grad_(True) for t in bad[:2]]
     torch.autograd.grad(fm.qk_norm_rotary(*leaves, *bad[4], *bad[5:]), leaves, bad[2:4])
     check(*problem(3, 1500, 9, 3, d, n, torch.bfloat16, torch.float32, seed=8), interleaved=interleaved)
+
+
+def test_no_second_derivative():
+    q, k, gq, gk, w, cos, sin, pos = problem(1, 6, 3, 2, 64, 32, torch.bfloat16, torch.float32, seed=9)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, *w)]
+    out = fm.qk_norm_rotary(*leaves, cos, sin, pos)
+    want = torch.autograd.grad(out, leaves, [gq, gk], retain_graph=True)
+    got = torch.autograd.grad(out, leaves, [gq, gk], create_graph=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            a.float().square().sum().backward(retain_graph=True)
