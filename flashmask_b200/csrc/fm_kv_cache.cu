@@ -15,25 +15,29 @@ struct KvWriteParams {
   int B, S;
 };
 
-// The part of a CTA's threads that walks rows of `upr` units of 8 values: thread = unit `col` of rows row0, row0 + step, ..
+// How TEAM threads walk rows of `upr` units of 8 values: thread = unit `col` of rows row0, row0 + step, ..
 struct RowWalk { int row0, step, col; };
-template <int THREADS>
+template <int TEAM>
 __device__ __forceinline__ RowWalk row_walk(int upr) {
-  const int step = THREADS / upr, row0 = threadIdx.x / upr;
-  return {row0 < step ? row0 : INT_MAX / 2, step, (int)threadIdx.x - row0 * upr};
+  const int tid = threadIdx.x & (TEAM - 1), step = TEAM / upr, row0 = tid / upr;
+  return {row0 < step ? row0 : INT_MAX / 2, step, tid - row0 * upr};
 }
 
-// One CTA = one page of one kv head, K or V (blockIdx.y = 2 * head + which), of the pages that the new tokens of sequence
-// blockIdx.z reach.  It reads its tokens once, keeps them in registers while the CTA finds the largest magnitude, and
+// One team (a CTA, or each of its warps) = one page of one kv head, K or V (2 * head + which), of the pages that the new tokens of
+// sequence blockIdx.z reach.  It reads its tokens once, keeps them in registers while it finds the largest magnitude, and
 // writes one byte for every two that it read.  Bound by HBM: 3 bytes a value.
 // A page that held tokens before (the write starts inside it) keeps its scale or grows it; where it grows, the payload
 // of the earlier tokens is rounded on the new grid.  Slots behind the last new token are left as they are.
 // VEC = units of 8 values that a thread holds.
-template <bool IS_BF16, bool INT8, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) : (VEC == 1 ? 1280 / THREADS : (VEC <= 8 ? 2 : 1))) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
-  constexpr int WARPS = THREADS / 32;
+// Threads on an SM.  64 registers for eight units spill less in int8 than in e4m3: 2 x 8192 tokens, 8 heads, d = 128, pages of 64 with
+// 1024 / 896 threads: int8 20.9 / 22.0 us, e4m3 23.3 / 19.3 us.
+constexpr int write_threads(bool int8, int vec, int threads) { return vec <= 4 ? 1280 : (vec > 8 ? 512 : (int8 || threads > 128 ? 1024 : 896)); }
+template <bool IS_BF16, bool INT8, int VEC, int THREADS, int TEAM>
+__global__ void __launch_bounds__(THREADS, write_threads(INT8, VEC, THREADS) / THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
+  constexpr int WARPS = TEAM / 32;
   __shared__ uint32_t s_max[WARPS];
-  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1, P = 1 << p.g.page_log2;
+  const int b = blockIdx.z, hw = TEAM == THREADS ? blockIdx.y : blockIdx.y * (THREADS / TEAM) + threadIdx.x / TEAM, which = hw & 1, h = hw >> 1, P = 1 << p.g.page_log2;
+  if (THREADS > TEAM && h >= p.g.Hkv) return;
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int start = p.start[b];
   if (n + min(start, 0) <= 0 || start > INT_MAX - p.S) return;  // (rows before position 0 are not written)
@@ -43,7 +47,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) 
   const int page = kv_page(p.g, p.table + b * p.g.table_stride, base);
   if (page < 0) return;
   const int w = p.width[which];
-  const RowWalk at = row_walk<THREADS>(w >> 3);
+  const RowWalk at = row_walk<TEAM>(w >> 3);
   const int lo = max(first - base, 0), hi = min(last - base + 1, P);       // slots [lo, hi) are new
   uint8_t* pay = p.pay[which] + ((size_t)page * p.g.Hkv + h) * P * w + at.col * 8;
   float* scale = p.scale[which] + (size_t)page * p.g.Hkv + h;
@@ -67,10 +71,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) 
   const int warp = threadIdx.x >> 5;
   auto largest = [&](uint32_t v) {
     v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) s_max[warp] = v;
-    __syncthreads();
+    if constexpr (WARPS > 1) {
+      if ((threadIdx.x & 31) == 0) s_max[warp] = v;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) v = max(v, s_max[i]);
+      for (int i = 0; i < WARPS; ++i) v = max(v, s_max[i]);
+    }
     return v;
   };
   top = largest(top);
@@ -88,7 +94,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) 
         if (u < INF) top = max(top, u); else v[c] = (v[c] & 0xffffu) | (INT8 ? 0u : 0x7fff0000u);
       }
     }
-    __syncthreads();
+    if constexpr (WARPS > 1) __syncthreads();
     top = largest(top);
   }
   int e = cache_exponent<INT8>(unpack2<IS_BF16>(top).x);
@@ -123,8 +129,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? (VEC <= 4 ? 10 : 8) 
       *to = v;
     }
   }
-  // every thread has read the old scale (the barriers above), so it can go
-  if (threadIdx.x == 0) *scale = INT8 && (bad || old_nan) ? __uint_as_float(0x7fffffffu) : exp2_int(e);
+  // every thread has read the old scale (it waited for the others' magnitudes), so it can go
+  if ((threadIdx.x & (TEAM - 1)) == 0) *scale = INT8 && (bad || old_nan) ? __uint_as_float(0x7fffffffu) : exp2_int(e);
 }
 
 struct KvReadParams {
@@ -136,13 +142,14 @@ struct KvReadParams {
   int B, S;
 };
 
-// dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  One CTA = the rows in one page of one kv
+// dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  One team (a CTA, or each of its warps) = the rows in one page of one kv
 // head, K and V: the page and its scales are looked up once, and a thread has READ_ILP units of 8 bytes of each in flight.
 // Bound by HBM: 3 bytes a value (2 x 8192 tokens of 8 heads, d = 128, 100 MB: 16 us, 6.3 TB/s; CTAs of 256 threads 18.5 us).
 constexpr int READ_ILP = 4;
-template <bool IS_BF16, bool INT8>
+template <bool IS_BF16, bool INT8, int TEAM>
 __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__ KvReadParams p) {
-  const int b = blockIdx.z, h = blockIdx.y, P = 1 << p.g.page_log2;
+  const int b = blockIdx.z, h = TEAM == 128 ? blockIdx.y : blockIdx.y * (128 / TEAM) + threadIdx.x / TEAM, P = 1 << p.g.page_log2;
+  if (TEAM < 128 && h >= p.g.Hkv) return;
   const int64_t start = p.start[b], base = ((start >> p.g.page_log2) + blockIdx.x) << p.g.page_log2;      // (rounds down below 0 too)
   const int len = kv_len(p.g, p.seqlens[b]);
   if (base >= start + p.S) return;
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
   const int lo = base < start ? (int)(start - base) : 0, hi = (int)min((int64_t)P, start + p.S - base);    // slots that are asked for
   const int valid = page >= 0 ? (int)min((int64_t)P, len - base) : 0;                                      // slots that hold tokens
   const size_t ph = (size_t)max(page, 0) * p.g.Hkv + h;
-  const RowWalk at[2] = {row_walk<128>(p.width[0] >> 3), row_walk<128>(p.width[1] >> 3)};
+  const RowWalk at[2] = {row_walk<TEAM>(p.width[0] >> 3), row_walk<TEAM>(p.width[1] >> 3)};
   float scale[2];
   const uint8_t* pay[2];
 #pragma unroll
@@ -260,18 +267,35 @@ static unsigned pages_of(int S, int page_size) { return (unsigned)(((int64_t)S +
 
 template <bool IS_BF16, bool INT8>
 static int launch_write(const KvWriteParams& p, int page_size, int width_max, cudaStream_t s) {
-  const dim3 grid(pages_of(p.S, page_size), 2 * p.g.Hkv, p.B);
+  const unsigned pages = pages_of(p.S, page_size), heads = 2 * p.g.Hkv;
+  const dim3 ctas(pages, heads, p.B), warps(pages, (heads + 3) / 4, p.B);
   const int upr = width_max / 8, rows = std::min(page_size, p.S);
   auto holds = [&](int threads, int vec) { return rows <= threads / upr * vec; };
-  // A few tokens: a CTA of 64 threads has a unit for each, and 2048 of them fit the chip at once.  Whole pages: CTAs of 128
-  // threads, eight to an SM (64 tokens of 128 values, 2 x 8192 of them with 8 heads: 17 us, 5.9 TB/s; 256 threads of four units,
-  // five to an SM: 20 us; 512 threads of two: 29 us).
-  if (holds(64, 1)) kv_write_kernel<IS_BF16, INT8, 1, 64><<<grid, 64, 0, s>>>(p);
-  else if (holds(256, 1)) kv_write_kernel<IS_BF16, INT8, 1, 256><<<grid, 256, 0, s>>>(p);
-  else if (holds(128, 4)) kv_write_kernel<IS_BF16, INT8, 4, 128><<<grid, 128, 0, s>>>(p);
-  else if (holds(128, 8)) kv_write_kernel<IS_BF16, INT8, 8, 128><<<grid, 128, 0, s>>>(p);
-  else if (holds(256, 8)) kv_write_kernel<IS_BF16, INT8, 8, 256><<<grid, 256, 0, s>>>(p);
-  else kv_write_kernel<IS_BF16, INT8, 16, 256><<<grid, 256, 0, s>>>(p);       // (128 tokens of 256 values: 4096 units; any width: 240 threads hold them)
+  // A few tokens or small pages: a warp for each, so that nobody waits for a CTA's start and its barrier (4 x 8192 tokens of 64 values,
+  // 8 heads, pages of 16: 20 us; a CTA of 256 threads each 74 us).  Else CTAs of 128 threads (64 tokens of 128 values, 2 x 8192 of them
+  // with 8 heads: 19 us, 5.2 TB/s; 256 threads of four units 3 us more, 512 threads of two 10 us more), and of 256 where those do
+  // not hold a page.
+  if (holds(32, 1)) kv_write_kernel<IS_BF16, INT8, 1, 128, 32><<<warps, 128, 0, s>>>(p);
+  else if (holds(32, 4)) kv_write_kernel<IS_BF16, INT8, 4, 128, 32><<<warps, 128, 0, s>>>(p);
+  else if (holds(32, 8)) kv_write_kernel<IS_BF16, INT8, 8, 128, 32><<<warps, 128, 0, s>>>(p);
+  else if (holds(128, 4)) kv_write_kernel<IS_BF16, INT8, 4, 128, 128><<<ctas, 128, 0, s>>>(p);
+  else if (holds(128, 8)) kv_write_kernel<IS_BF16, INT8, 8, 128, 128><<<ctas, 128, 0, s>>>(p);
+  else if (holds(256, 8)) kv_write_kernel<IS_BF16, INT8, 8, 256, 256><<<ctas, 256, 0, s>>>(p);
+  else kv_write_kernel<IS_BF16, INT8, 16, 256, 256><<<ctas, 256, 0, s>>>(p);       // (128 tokens of 256 values: 4096 units; any width: 240 threads hold them)
+  count_launches(1);
+  FM_CUDA_TRY(cudaGetLastError());
+  return FM_OK;
+}
+
+// A warp for a page's rows where two rounds of it are enough: 128 threads would not have READ_ILP units each (4 x 8192 tokens of 64
+// values, pages of 16: 16 us; a CTA each 33 us).
+template <bool IS_BF16, bool INT8>
+static int launch_read(const KvReadParams& p, int page_size, cudaStream_t s) {
+  const unsigned pages = pages_of(p.S, page_size);
+  if (std::min(page_size, p.S) <= 32 / (std::max(p.width[0], p.width[1]) / 8) * 2 * READ_ILP)
+    kv_read_kernel<IS_BF16, INT8, 32><<<dim3(pages, (p.g.Hkv + 3) / 4, p.B), 128, 0, s>>>(p);
+  else
+    kv_read_kernel<IS_BF16, INT8, 128><<<dim3(pages, p.g.Hkv, p.B), 128, 0, s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   return FM_OK;
@@ -323,14 +347,10 @@ extern "C" FM_API int fm_kv_read(const fm_kv_cache* c, const fm_kv_args* a, void
   p.width[0] = c->d; p.width[1] = c->dv;
   p.table = a->page_table; p.start = a->start; p.seqlens = a->seqlens;
   p.B = a->B; p.S = a->S;
-  const dim3 grid(pages_of(a->S, c->page_size), c->Hkv, a->B);
   const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
   cudaStream_t s = (cudaStream_t)stream;
-  if (bf) { if (i8) kv_read_kernel<true, true><<<grid, 128, 0, s>>>(p); else kv_read_kernel<true, false><<<grid, 128, 0, s>>>(p); }
-  else { if (i8) kv_read_kernel<false, true><<<grid, 128, 0, s>>>(p); else kv_read_kernel<false, false><<<grid, 128, 0, s>>>(p); }
-  count_launches(1);
-  FM_CUDA_TRY(cudaGetLastError());
-  return FM_OK;
+  if (bf) return i8 ? launch_read<true, true>(p, c->page_size, s) : launch_read<true, false>(p, c->page_size, s);
+  return i8 ? launch_read<false, true>(p, c->page_size, s) : launch_read<false, false>(p, c->page_size, s);
 }
 
 extern "C" FM_API int fm_kv_bounds(const fm_kv_cache* c, const fm_kv_args* a, int cols, int32_t* shift, int32_t* bounds, void* stream) {
