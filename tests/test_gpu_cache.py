@@ -127,6 +127,14 @@ def test_write_is_exact_and_reads_back(kind, dtype, page, d, dv, H):
 
 
 @pytest.mark.parametrize("kind", [E4M3, INT8])
+@pytest.mark.parametrize("page,d,dv,H", [(64, 32, 32, 3), (32, 64, 64, 5), (16, 192, 128, 3), (16, 256, 256, 3), (64, 64, 64, 1), (128, 128, 128, 1), (64, 256, 256, 1),
+                                         (64, 112, 16, 2)])
+def test_pages_that_warps_or_ctas_take(kind, page, d, dv, H):
+    """Pages from a warp's share to a CTA's, heads that do not fill a CTA of warps, widths that leave lanes over."""
+    test_write_is_exact_and_reads_back(kind, torch.bfloat16, page, d, dv, H)
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8])
 def test_tokens_appended_one_by_one(kind):
     """Scales that grow while a page fills, from tiny to large and back, and stay when they need not."""
     H, d, page = 2, 32, 16
