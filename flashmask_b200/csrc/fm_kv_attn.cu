@@ -386,8 +386,9 @@ __global__ void __launch_bounds__(KV_WARPS * 32, KvCfg<DK, VC, NT>::CTAS) kv_att
     if (turn) {
       // the next item's queries (row g of tile `warp`) are on their way while the last one's sums are joined
       last = seg;
-      if (i < 0) seg = ahead.of_lane(0);
-      else if (i < n_units) seg = segment(u_begin + i);
+      const int at = max(i, 0);
+      if ((at + STAGES - 2) >> 4 == at >> 4) seg = ahead.of_lane(2 * (at & 15));      // (looked up with the units of its round)
+      else if (at < n_units) seg = segment(u_begin + at);
       const int row = seg.row0 + warp * 8 + g, qi = row / p.G;
       const bool on = warp < NT && i < n_units && qi < p.S;
       const uint16_t* src = p.q + seg.b * p.qs[0] + qi * p.qs[1] + ((int64_t)seg.h * p.G + row - qi * p.G) * p.qs[2];
