@@ -753,15 +753,25 @@ int kv_geometry(const fm_kv_cache* c, const fm_kv_args* a, KvGeom* g);
 
 constexpr int KV_MAX_B = 1024;                      // first units of the sequences are kept in shared memory
 
+template <class Cfg>
+static size_t kv_smem(int B) { return Cfg::FIXED + (size_t)std::max(B + 1, KV_WARPS * 33) * 4; }        // with the first units of the sequences
+// CTAs that an SM holds (228 KB, 1 KB of each the system's).  More would run behind the others, with an equal share of the work: 1024
+// sequences of 64 keys, d = 64, 92 us with a fourth CTA that does not fit, 72 us without.
+template <class Cfg>
+static int kv_ctas(int B) {
+  static_assert(Cfg::CTAS > 1 || Cfg::FIXED + (KV_MAX_B + 1) * 4 <= 227 * 1024, "one CTA always fits");
+  return (kv_smem<Cfg>(B) + 1024) * Cfg::CTAS <= 228 * 1024 ? Cfg::CTAS : Cfg::CTAS - 1;
+}
+
 struct KvAttnPlan { int vc, nt, n_cta; size_t bytes; };
 static KvAttnPlan kv_attn_plan(const fm_kv_cache* c, const fm_kv_args* a) {
   KvAttnPlan pl;
   const int64_t rows = (int64_t)a->S * (a->Hq / c->Hkv);
   pl.vc = c->dv <= 64 && c->d <= 64 ? 8 : (c->dv <= 128 ? 16 : 32);
   pl.nt = rows <= 8 || pl.vc == 32 ? 1 : (rows <= 16 || c->d > 128 ? 2 : (rows <= 24 ? 3 : 4));
-  pl.n_cta = sm_count() * (pl.vc > 16 ? KvCfg<4, 32, 1>::CTAS : c->d > 128 ? KvCfg<3, 16, 1>::CTAS
-             : pl.vc == 16 ? (pl.nt == 1 ? KvCfg<2, 16, 1>::CTAS : pl.nt == 2 ? KvCfg<2, 16, 2>::CTAS : pl.nt == 3 ? KvCfg<2, 16, 3>::CTAS : KvCfg<2, 16, 4>::CTAS)
-                           : (pl.nt == 1 ? KvCfg<1, 8, 1>::CTAS : pl.nt == 2 ? KvCfg<1, 8, 2>::CTAS : pl.nt == 3 ? KvCfg<1, 8, 3>::CTAS : KvCfg<1, 8, 4>::CTAS));
+  pl.n_cta = sm_count() * (pl.vc > 16 ? kv_ctas<KvCfg<4, 32, 1>>(a->B) : c->d > 128 ? (pl.nt == 1 ? kv_ctas<KvCfg<3, 16, 1>>(a->B) : kv_ctas<KvCfg<3, 16, 2>>(a->B))
+             : pl.vc == 16 ? (pl.nt == 1 ? kv_ctas<KvCfg<2, 16, 1>>(a->B) : pl.nt == 2 ? kv_ctas<KvCfg<2, 16, 2>>(a->B) : pl.nt == 3 ? kv_ctas<KvCfg<2, 16, 3>>(a->B) : kv_ctas<KvCfg<2, 16, 4>>(a->B))
+                           : (pl.nt == 1 ? kv_ctas<KvCfg<1, 8, 1>>(a->B) : pl.nt == 2 ? kv_ctas<KvCfg<1, 8, 2>>(a->B) : pl.nt == 3 ? kv_ctas<KvCfg<1, 8, 3>>(a->B) : kv_ctas<KvCfg<1, 8, 4>>(a->B)));
   pl.bytes = (size_t)2 * pl.n_cta * pl.nt * 8 * (8 * pl.vc + 2) * sizeof(float);
   return pl;
 }
@@ -770,10 +780,9 @@ template <int DK, int VC, int NT, bool INT8, bool FULL>
 static int launch_kv_attn(const KvAttnParams& p, cudaStream_t s) {
   using Cfg = KvCfg<DK, VC, NT>;
   auto kern = kv_attn_kernel<DK, VC, NT, INT8, FULL>;
-  const size_t smem = Cfg::FIXED + (size_t)std::max(p.B + 1, KV_WARPS * 33) * 4;      // first units of the sequences
   static std::atomic<uint64_t> done{0};
-  FM_CUDA_TRY(allow_smem(kern, Cfg::FIXED + (KV_MAX_B + 1) * 4, done));
-  kern<<<p.n_cta, KV_WARPS * 32, smem, s>>>(p);
+  FM_CUDA_TRY(allow_smem(kern, (int)kv_smem<Cfg>(KV_MAX_B), done));
+  kern<<<p.n_cta, KV_WARPS * 32, kv_smem<Cfg>(p.B), s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   // (a row of up to 8 parts is one warp's)

@@ -315,6 +315,15 @@ def test_large_scores_and_scales():
     check_attention(f, q[:, :, 1:2])
 
 
+@pytest.mark.parametrize("d,G", [(64, 1), (64, 9), (128, 2)])
+def test_as_many_sequences_as_a_call_takes(d, G):
+    """1024 short ones and a long one among them, which is cut."""
+    lens = [(i * 29) % 40 for i in range(1024)]
+    lens[500] = 1500
+    f = Filled(lens, 1, d, d, E4M3, 16, seed=23)
+    check_attention(f, rand_q(1024, 1, G, d, seed=24))
+
+
 @pytest.mark.parametrize("kind", [E4M3, INT8])
 @pytest.mark.parametrize("S,window", [(1, None), (3, None), (3, 24)])
 def test_nan_where_nobody_looks(kind, S, window):
