@@ -92,9 +92,10 @@ def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, page_table:
     without ``causal``.  Rows that see nothing, padding among them, give 0 and an lse of -inf (of the sink's logit with
     ``sink``, one per query head, which joins every denominator).
 
-    Up to 96 rows for each kv head (S x Hq / Hkv) the pages are read as they are, and neither ``seqlens`` nor anything else is
-    needed on the host, so the call can be captured into a CUDA graph with lengths that change between replays.  With more
-    rows the tokens are read back into 16-bit tensors of ``max_seqlen`` positions (an upper bound of ``seqlens``; without it the
+    Up to 96 rows for each kv head (S x Hq / Hkv; more with head dims above 128 and few kv heads in all sequences together) the pages
+    are read as they are, and neither ``seqlens`` nor anything else is needed on the host, so the call can be captured into a CUDA graph
+    with lengths that change between replays.  With more rows the tokens are read back into 16-bit tensors of ``max_seqlen`` positions
+    (an upper bound of ``seqlens``; without it the
     whole page table, as long as that takes no more than 2 GiB) and go through the dense forward.  At most 1024 sequences."""
     if sink is not None and learnable_sink is not None:
         raise ValueError("pass either sink or learnable_sink, not both")

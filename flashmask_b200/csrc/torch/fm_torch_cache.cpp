@@ -256,9 +256,13 @@ std::pair<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Tens
 
 // Rows (queries x heads of a group) up to which the cache is read by the kernel for few rows.  Beyond, the tokens are
 // read back once into dense 16-bit tensors and the dense forward, which feeds the tensor cores, takes the call.  Measured, 32 / 8
-// heads, d = 128: 64 rows 37 us and 68 rows 48 us for 16384 keys (128 rows: 54), 54 and 78 us for 8 x 4096 (82), 118 and 165
-// us for 64 x 1024, where the kernel's time goes with the number of 32-row tiles and the other's hardly with the rows.
-constexpr int64_t kFewRows = 96;
+// heads, d = 128: 96 rows 41 us and 100 rows 50 us for 16384 keys, 70 and 77 us for 8 x 4096, 111 and 98 us for 64 x 512: the
+// kernel's time goes with the number of 32-row tiles and the other's hardly with the rows.
+// Head dims above 128: the dense forward does not deal a row block's K tiles to several CTAs, so its time does not depend on
+// the rows while these leave SMs idle, and the kernel's goes with all rows of the call.  Kernel and dense forward, us: 16384 keys, 32 / 8 heads,
+// d = 192: 112 rows 54 and 277, 640 rows 243 and 372; 4 x 4096: 160 rows 73 and 97; 16384 keys, 16 / 4 heads, d = 256: 112 rows 87 and
+// 185, 224 rows 164 and 185.
+int64_t few_rows(int64_t d, int64_t kv_heads) { return std::max<int64_t>(96, d <= 128 ? 0 : (d <= 192 ? 5400 : 900) / std::max<int64_t>(kv_heads, 1)); }
 // Without an upper bound of the lengths the dense tensors cover the whole page table, which may be far wider than the
 // sequences are long: beyond this many bytes the kernel for few rows, which needs none, keeps the call.
 constexpr int64_t kNoBound = (int64_t)1 << 40, kMostDense = (int64_t)2 << 30;
@@ -295,7 +299,7 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
   int64_t cols = std::min<int64_t>(max_seqlen, (int64_t)a.max_pages * f.page_size);
   cols = std::max<int64_t>(lengths ? cols + S : cols, S);
   const bool bounded = max_seqlen < kNoBound || B * cols * f.Hkv * (f.d + f.dv) * 2 <= kMostDense;
-  if (S * (Hq / f.Hkv) > kFewRows && B > 0 && bounded) {
+  if (S * (Hq / f.Hkv) > few_rows(f.d, B * f.Hkv) && B > 0 && bounded) {
     const Tensor shift = fresh({B}, at::kInt, ck), bounds = fresh({B, 1, cols, causal ? 1 : 2}, at::kInt, ck);
     check(fm_kv_bounds(&f, &a, (int)cols, shift.data_ptr<int>(), bounds.data_ptr<int>(), stream), "fm_kv_bounds");
     const Tensor k = fresh({B, cols, f.Hkv, f.d}, query.scalar_type(), ck), v = fresh({B, cols, f.Hkv, f.dv}, query.scalar_type(), ck);

@@ -315,6 +315,14 @@ def test_large_scores_and_scales():
     check_attention(f, q[:, :, 1:2])
 
 
+@pytest.mark.parametrize("d,dv,S", [(192, 128, 130), (192, 128, 230), (256, 256, 32), (256, 256, 40)])
+def test_many_rows_of_wide_heads(d, dv, S):
+    """Rows on both sides of where the dense forward takes over (three sequences of 2 kv heads: 900 rows | 150 rows)."""
+    f = Filled([300, 37, 150], 2, d, dv, E4M3, 32, seed=25)
+    check_attention(f, rand_q(3, S, 8, d, seed=26), q_lengths=[S, 20, S - 9])
+    check_attention(f, rand_q(3, S, 8, d, seed=27), causal=False)
+
+
 @pytest.mark.parametrize("d,G", [(64, 1), (64, 9), (128, 2)])
 def test_as_many_sequences_as_a_call_takes(d, G):
     """1024 short ones and a long one among them, which is cut."""
