@@ -19,8 +19,9 @@ struct KvWriteParams {
 struct RowWalk { int row0, step, col; };
 template <int TEAM>
 __device__ __forceinline__ RowWalk row_walk(int upr) {
-  const int tid = threadIdx.x & (TEAM - 1), step = TEAM / upr, row0 = tid / upr;
-  return {row0 < step ? row0 : INT_MAX / 2, step, tid - row0 * upr};
+  const unsigned tid = TEAM == 32 ? threadIdx.x & 31 : threadIdx.x;
+  const int step = TEAM / upr, row0 = tid / upr;
+  return {row0 < step ? row0 : INT_MAX / 2, step, (int)tid - row0 * upr};
 }
 
 // One team (a CTA, or each of its warps) = one page of one kv head, K or V (2 * head + which), of the pages that the new tokens of
@@ -31,9 +32,9 @@ __device__ __forceinline__ RowWalk row_walk(int upr) {
 // VEC = units of 8 values that a thread holds.
 // Threads on an SM.  64 registers for eight units spill less in int8 than in e4m3: 2 x 8192 tokens, 8 heads, d = 128, pages of 64 with
 // 1024 / 896 threads: int8 20.9 / 22.0 us, e4m3 23.3 / 19.3 us.
-constexpr int write_threads(bool int8, int vec, int threads) { return vec <= 4 ? 1280 : (vec > 8 ? 512 : (int8 || threads > 128 ? 1024 : 896)); }
+constexpr int write_threads(bool int8, int vec) { return vec <= 4 ? 1280 : (vec > 8 ? 512 : (int8 ? 1024 : 896)); }
 template <bool IS_BF16, bool INT8, int VEC, int THREADS, int TEAM>
-__global__ void __launch_bounds__(THREADS, write_threads(INT8, VEC, THREADS) / THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
+__global__ void __launch_bounds__(THREADS, write_threads(INT8, VEC) / THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
   constexpr int WARPS = TEAM / 32;
   __shared__ uint32_t s_max[WARPS];
   const int b = blockIdx.z, hw = TEAM == THREADS ? blockIdx.y : blockIdx.y * (THREADS / TEAM) + threadIdx.x / TEAM, which = hw & 1, h = hw >> 1, P = 1 << p.g.page_log2;
