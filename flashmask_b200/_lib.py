@@ -76,6 +76,7 @@ class KvArgs(C.Structure):
         ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("sink", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("q_stride", I64x3), ("k_stride", I64x3), ("v_stride", I64x3),
+        ("marks", C.c_void_p),
     ]
 
 
@@ -131,6 +132,7 @@ SIGNATURES = {
     "fm_kv_attention_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvArgs)]),
     "fm_kv_attention": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_void_p]),
     "fm_kv_bounds": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "fm_kv_nan_rows": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvArgs), C.c_void_p]),
 }
 
 _lib = None

@@ -90,7 +90,8 @@ def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, page_table:
     ``n = q_lengths[b]`` query rows (S without ``q_lengths``; the rest is padding), and row i stands at position
     ``seqlens[b] - n + i``.  It sees the positions up to its own, with ``window_size`` the last ``window_size`` of them, or all
     without ``causal``.  Rows that see nothing, padding among them, give 0 and an lse of -inf (of the sink's logit with
-    ``sink``, one per query head, which joins every denominator).
+    ``sink``, one per query head, which joins every denominator).  A NaN reaches the rows that see its token and no others: a
+    NaN value in e4m3 its column, a NaN key, and in int8 a page whose scale is NaN, the whole row and its lse.
 
     Up to 96 rows for each kv head (S x Hq / Hkv; more with head dims above 128 and few kv heads in all sequences together) the pages
     are read as they are, and neither ``seqlens`` nor anything else is needed on the host, so the call can be captured into a CUDA graph

@@ -119,9 +119,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   return r;
 }
 
-// 0x80 in every byte of w that is an e4m3 NaN (0x7f, 0xff).
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
 // What a range of units of one item is: the item, and which of its keys.
 struct KvSegment {
   int b, h, row0, units, u0, u1, key0;

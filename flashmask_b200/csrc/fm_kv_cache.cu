@@ -140,14 +140,17 @@ struct KvReadParams {
   uint16_t* dst[2];
   int width[2];
   const int32_t* table; const int32_t* start; const int32_t* seqlens;
+  int32_t* marks;                                                // [B, Hkv] (MARK)
   int B, S;
 };
 
 // dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  One team (a CTA, or each of its warps) = the rows in one page of one kv
 // head, K and V: the page and its scales are looked up once, and a thread has READ_ILP units of 8 bytes of each in flight.
 // Bound by HBM: 3 bytes a value (2 x 8192 tokens of 8 heads, d = 128, 100 MB: 16 us, 6.3 TB/s; CTAs of 256 threads 18.5 us).
+// MARK: for a dense forward, whose P V would take 0 * NaN into rows that do not see the token.  What is NaN comes as 0, and
+// marks[b, h] says that there was some; kv_nan_kernel brings it to the rows that see it.
 constexpr int READ_ILP = 4;
-template <bool IS_BF16, bool INT8, int TEAM>
+template <bool IS_BF16, bool INT8, int TEAM, bool MARK>
 __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__ KvReadParams p) {
   const int b = blockIdx.z, h = TEAM == 128 ? blockIdx.y : blockIdx.y * (128 / TEAM) + threadIdx.x / TEAM, P = 1 << p.g.page_log2;
   if (TEAM < 128 && h >= p.g.Hkv) return;
@@ -165,6 +168,12 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
   for (int x = 0; x < 2; ++x) {
     scale[x] = page >= 0 ? __ldg(p.scale[x] + ph) : 0.f;
     pay[x] = p.pay[x] + ph * P * p.width[x] + at[x].col * 8;
+  }
+  bool found = false;
+  if constexpr (MARK) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      if (scale[x] != scale[x]) { scale[x] = 0.f; found = lo < min(hi, valid); }
   }
   for (int row0 = lo; row0 < hi; row0 += READ_ILP * min(at[0].step, at[1].step)) {
     uint2 v[2][READ_ILP];
@@ -185,6 +194,14 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
         const int row = row0 + at[x].row0 + i * at[x].step;
         if (row >= upto) break;
         float a[4], c[4];
+        if constexpr (MARK && !INT8) {
+          const uint32_t n0 = nan_bytes(v[x][i].x), n1 = nan_bytes(v[x][i].y);
+          if ((n0 | n1) != 0) {
+            found = true;
+            v[x][i].x &= ~((n0 >> 7) * 0xffu);
+            v[x][i].y &= ~((n1 >> 7) * 0xffu);
+          }
+        }
         payload_f32<INT8>(v[x][i].x, a);
         payload_f32<INT8>(v[x][i].y, c);
         const float sc = row < valid ? scale[x] : 0.f;            // (a NaN scale is no token's)
@@ -199,6 +216,7 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
       }
     }
   }
+  if (MARK && found) p.marks[(int64_t)b * p.g.Hkv + h] = 1;
 }
 
 // Column bounds that make a dense causal forward over the read-back tokens see what the cache's rows see.  Column c
@@ -208,7 +226,7 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
 struct KvBoundsParams {
   KvGeom g;
   const int32_t* seqlens; const int32_t* lengths; const int32_t* table;
-  int32_t* shift; int32_t* bounds;
+  int32_t* shift; int32_t* bounds; int32_t* marks;              // marks: zeroed, or NULL
   int B, Sq, cols, causal, window;
 };
 __global__ void __launch_bounds__(256) kv_bounds_kernel(const KvBoundsParams p) {
@@ -219,6 +237,8 @@ __global__ void __launch_bounds__(256) kv_bounds_kernel(const KvBoundsParams p) 
   // the first row stands at len - n and, bottom-right aligned, sees the columns up to cols - Sq
   const int shift = len - n - (p.cols - p.Sq);
   if (c == 0) p.shift[b] = shift;
+  if (p.marks && blockIdx.x == 0)
+    for (int h = threadIdx.x; h < p.g.Hkv; h += 256) p.marks[(int64_t)b * p.g.Hkv + h] = 0;
   if (c >= p.cols) return;
   const int pos = shift + c;
   int end = 0;
@@ -229,6 +249,101 @@ __global__ void __launch_bounds__(256) kv_bounds_kernel(const KvBoundsParams p) 
   end = max(end, 0);
   if (p.causal) p.bounds[(int64_t)b * p.cols + c] = end;
   else reinterpret_cast<int2*>(p.bounds)[(int64_t)b * p.cols + c] = make_int2(end, 0);
+}
+
+// NaN for the rows of a dense forward that see a token whose key or value is none (it got 0 in its place): the whole row and its
+// lse where a key or a page's scale is NaN, the value's column where a value in e4m3 is.  And an lse of NaN for the other rows
+// of NaN, those of a NaN query, which the dense forward leaves with -inf.
+// One CTA = up to NAN_ROWS query rows of a sequence and kv head.  Nearly always there is no mark, and a CTA reads its rows' lse and leaves (512
+// rows, 32 / 8 heads: 128 CTAs, one round trip to memory).  With a mark its warps walk the groups of 16 tokens that one of the rows sees, lanes
+// side by side along the payload; tokens that all rows see, nearly all, cost no work per row.
+struct KvNanParams {
+  KvGeom g;
+  const uint8_t* pay[2]; const float* scale[2];
+  int width[2];
+  const int32_t* table; const int32_t* seqlens; const int32_t* lengths; const int32_t* marks;
+  uint16_t* o; float* lse;
+  int B, S, Hq, G, causal, window;
+};
+constexpr int NAN_ROWS = 32, NAN_WORDS = 64;                     // (64 words of 4 values: 256 is the widest head)
+template <bool IS_BF16, bool INT8>
+__global__ void __launch_bounds__(256) kv_nan_kernel(const __grid_constant__ KvNanParams p) {
+  __shared__ uint32_t s_cols[NAN_ROWS + 1][NAN_WORDS];           // 0x80 in the bytes of columns that are NaN; the last row: for every row
+  __shared__ int s_row[NAN_ROWS + 1];                            // the whole row is
+  constexpr uint32_t INF = IS_BF16 ? 0x7f80u : 0x7c00u;
+  const int b = blockIdx.z, h = blockIdx.y, i0 = blockIdx.x * NAN_ROWS, rows = min(NAN_ROWS, p.S - i0);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dv = p.width[1], words = dv / 4;
+  const float nan = __uint_as_float(0x7fffffffu);
+  auto head_row = [&](int x, int& hq, int& i) { hq = h * p.G + x / rows; i = i0 + x % rows; };
+  grid_dep_wait();
+  for (int x = tid; x < rows * p.G; x += 256) {
+    int hq, i;
+    head_row(x, hq, i);
+    float* lse = p.lse + ((int64_t)b * p.Hq + hq) * p.S + i;
+    if (__ldcg(lse) == -INFINITY && (__ldcg(p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * dv) & 0x7fffu) > INF) *lse = nan;
+  }
+  if (__ldcg(p.marks + (int64_t)b * p.g.Hkv + h) == 0) return;
+  const int len = kv_len(p.g, p.seqlens[b]), n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
+  const int live = min(rows, n - i0);                            // rows that are queries
+  if (live <= 0) return;
+  // keys [row_lo(r), row_hi(r)) of row r
+  const int p0 = len - n + i0;
+  auto row_lo = [&](int r) { return p.window > 0 ? max(p0 + r + 1 - p.window, 0) : 0; };
+  auto row_hi = [&](int r) { return p.causal ? max(p0 + r + 1, 0) : len; };
+  for (int x = tid; x < (NAN_ROWS + 1) * NAN_WORDS; x += 256) s_cols[x / NAN_WORDS][x % NAN_WORDS] = 0;
+  if (tid <= NAN_ROWS) s_row[tid] = 0;
+  __syncthreads();
+  const int lo = row_lo(0), hi = row_hi(live - 1), all_lo = row_lo(live - 1), all_hi = row_hi(0);      // one row sees [lo, hi), all see [all_lo, all_hi)
+  for (int g0 = (lo >> 4) + warp; g0 < (hi + 15) >> 4; g0 += 8) {
+    const int page = kv_page(p.g, p.table + b * p.g.table_stride, g0 << 4);
+    if (page < 0) continue;
+    const size_t ph = (size_t)page * p.g.Hkv + h;
+    const float ks = p.scale[0][ph], vs = p.scale[1][ph];
+    const bool dead = ks != ks || vs != vs;
+    if (INT8 && !dead) continue;
+    const int slot = (g0 << 4) & ((1 << p.g.page_log2) - 1);
+#pragma unroll 4
+    for (int j = 0; j < 16; ++j) {
+      const int pos = (g0 << 4) + j;
+      const bool seen = pos >= lo && pos < hi;
+      const uint8_t *k = p.pay[0] + ((ph << p.g.page_log2) + slot + j) * p.width[0], *v = p.pay[1] + ((ph << p.g.page_log2) + slot + j) * dv;
+      uint32_t in_k = 0, in_v[NAN_WORDS / 32] = {};
+      if (!INT8 && seen) {
+#pragma unroll
+        for (int c = 0; c < NAN_WORDS / 32; ++c) {
+          const int w = lane + 32 * c;
+          if (4 * w < p.width[0]) in_k |= nan_bytes(*reinterpret_cast<const uint32_t*>(k + 4 * w));
+          if (w < words) in_v[c] = nan_bytes(*reinterpret_cast<const uint32_t*>(v + 4 * w));
+        }
+      }
+      const bool whole = seen && (dead || __any_sync(0xffffffffu, in_k != 0));
+      uint32_t any_v = 0;
+#pragma unroll
+      for (int c = 0; c < NAN_WORDS / 32; ++c) any_v |= in_v[c];
+      if (!whole && !__any_sync(0xffffffffu, any_v != 0)) continue;
+      const bool all = pos >= all_lo && pos < all_hi;
+      for (int r = all ? NAN_ROWS : 0; r < (all ? NAN_ROWS + 1 : live); ++r) {
+        if (!all && (pos < row_lo(r) || pos >= row_hi(r))) continue;
+        if (whole && lane == 0) s_row[r] = 1;
+#pragma unroll
+        for (int c = 0; c < NAN_WORDS / 32; ++c)
+          if (in_v[c]) atomicOr(&s_cols[r][lane + 32 * c], in_v[c]);
+      }
+    }
+  }
+  __syncthreads();
+  for (int x = warp; x < live * p.G; x += 8) {
+    const int r = x % live, i = i0 + r, hq = h * p.G + x / live;
+    const bool whole = s_row[r] != 0 || s_row[NAN_ROWS] != 0;
+    uint16_t* o = p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * dv;
+    for (int w = lane; w < words; w += 32) {
+      const uint32_t cols = whole ? 0x80808080u : s_cols[r][w] | s_cols[NAN_ROWS][w];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (cols >> (8 * c + 7) & 1u) o[4 * w + c] = 0x7fffu;
+    }
+    if (whole && lane == 0) p.lse[((int64_t)b * p.Hq + hq) * p.S + i] = nan;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -290,16 +405,21 @@ static int launch_write(const KvWriteParams& p, int page_size, int width_max, cu
 
 // A warp for a page's rows where two rounds of it are enough: 128 threads would not have READ_ILP units each (4 x 8192 tokens of 64
 // values, pages of 16: 16 us; a CTA each 33 us).
-template <bool IS_BF16, bool INT8>
+template <bool IS_BF16, bool INT8, bool MARK>
 static int launch_read(const KvReadParams& p, int page_size, cudaStream_t s) {
   const unsigned pages = pages_of(p.S, page_size);
   if (std::min(page_size, p.S) <= 32 / (std::max(p.width[0], p.width[1]) / 8) * 2 * READ_ILP)
-    kv_read_kernel<IS_BF16, INT8, 32><<<dim3(pages, (p.g.Hkv + 3) / 4, p.B), 128, 0, s>>>(p);
+    kv_read_kernel<IS_BF16, INT8, 32, MARK><<<dim3(pages, (p.g.Hkv + 3) / 4, p.B), 128, 0, s>>>(p);
   else
-    kv_read_kernel<IS_BF16, INT8, 128><<<dim3(pages, p.g.Hkv, p.B), 128, 0, s>>>(p);
+    kv_read_kernel<IS_BF16, INT8, 128, MARK><<<dim3(pages, p.g.Hkv, p.B), 128, 0, s>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
   return FM_OK;
+}
+template <bool MARK>
+static int dispatch_read(const KvReadParams& p, bool bf, bool i8, int page_size, cudaStream_t s) {
+  if (bf) return i8 ? launch_read<true, true, MARK>(p, page_size, s) : launch_read<true, false, MARK>(p, page_size, s);
+  return i8 ? launch_read<false, true, MARK>(p, page_size, s) : launch_read<false, false, MARK>(p, page_size, s);
 }
 
 }  // namespace fm
@@ -346,12 +466,11 @@ extern "C" FM_API int fm_kv_read(const fm_kv_cache* c, const fm_kv_args* a, void
   p.pay[0] = (const uint8_t*)c->k; p.pay[1] = (const uint8_t*)c->v; p.scale[0] = c->k_scale; p.scale[1] = c->v_scale;
   p.dst[0] = (uint16_t*)a->k_out; p.dst[1] = (uint16_t*)a->v_out;
   p.width[0] = c->d; p.width[1] = c->dv;
-  p.table = a->page_table; p.start = a->start; p.seqlens = a->seqlens;
+  p.table = a->page_table; p.start = a->start; p.seqlens = a->seqlens; p.marks = a->marks;
   p.B = a->B; p.S = a->S;
   const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
   cudaStream_t s = (cudaStream_t)stream;
-  if (bf) return i8 ? launch_read<true, true>(p, c->page_size, s) : launch_read<true, false>(p, c->page_size, s);
-  return i8 ? launch_read<false, true>(p, c->page_size, s) : launch_read<false, false>(p, c->page_size, s);
+  return p.marks ? dispatch_read<true>(p, bf, i8, c->page_size, s) : dispatch_read<false>(p, bf, i8, c->page_size, s);
 }
 
 extern "C" FM_API int fm_kv_bounds(const fm_kv_cache* c, const fm_kv_args* a, int cols, int32_t* shift, int32_t* bounds, void* stream) {
@@ -364,10 +483,31 @@ extern "C" FM_API int fm_kv_bounds(const fm_kv_cache* c, const fm_kv_args* a, in
   FM_REQUIRE(a->seqlens && shift && bounds, FM_ERR_INVALID_ARGUMENT, "fm_kv_bounds: seqlens, shift or bounds is NULL");
   FM_REQUIRE(((uintptr_t)bounds & 7) == 0, FM_ERR_INVALID_ARGUMENT, "fm_kv_bounds: bounds is not 8-byte aligned");
   p.seqlens = a->seqlens; p.lengths = a->lengths; p.table = a->page_table;
-  p.shift = shift; p.bounds = bounds;
+  p.shift = shift; p.bounds = bounds; p.marks = a->marks;
   p.B = a->B; p.Sq = a->S; p.cols = cols; p.causal = a->causal; p.window = a->window;
   kv_bounds_kernel<<<dim3((unsigned)((cols + 255) / 256), a->B), 256, 0, (cudaStream_t)stream>>>(p);
   count_launches(1);
   FM_CUDA_TRY(cudaGetLastError());
+  return FM_OK;
+}
+
+extern "C" FM_API int fm_kv_nan_rows(const fm_kv_cache* c, const fm_kv_args* a, void* stream) {
+  KvNanParams p;
+  const int rc = kv_geometry(c, a, &p.g);
+  if (rc) return rc;
+  FM_REQUIRE(a->Hq > 0 && a->Hq % c->Hkv == 0, FM_ERR_INVALID_ARGUMENT, "fm_kv_nan_rows: Hq=%d is no multiple of Hkv=%d", a->Hq, c->Hkv);
+  FM_REQUIRE(a->window >= 0 && (a->causal || a->window == 0), FM_ERR_INVALID_ARGUMENT, "fm_kv_nan_rows: window %d (causal %d)", a->window, a->causal);
+  if (a->B == 0 || a->S == 0) return FM_OK;
+  FM_REQUIRE(a->o && a->lse && a->seqlens && a->marks, FM_ERR_INVALID_ARGUMENT, "fm_kv_nan_rows: o, lse, seqlens or marks is NULL");
+  p.pay[0] = (const uint8_t*)c->k; p.pay[1] = (const uint8_t*)c->v; p.scale[0] = c->k_scale; p.scale[1] = c->v_scale;
+  p.width[0] = c->d; p.width[1] = c->dv;
+  p.table = a->page_table; p.seqlens = a->seqlens; p.lengths = a->lengths; p.marks = a->marks;
+  p.o = (uint16_t*)a->o; p.lse = a->lse;
+  p.B = a->B; p.S = a->S; p.Hq = a->Hq; p.G = a->Hq / c->Hkv;
+  p.causal = a->causal; p.window = std::min(a->window, 1 << 30);
+  const bool bf = a->dtype == FM_DTYPE_BF16, i8 = c->dtype == FM_CACHE_INT8;
+  auto kern = bf ? (i8 ? kv_nan_kernel<true, true> : kv_nan_kernel<true, false>) : (i8 ? kv_nan_kernel<false, true> : kv_nan_kernel<false, false>);
+  FM_CUDA_TRY(launch_dependent(kern, dim3((unsigned)((a->S + NAN_ROWS - 1) / NAN_ROWS), c->Hkv, a->B), dim3(256), 0, (cudaStream_t)stream, p));
+  count_launches(1);
   return FM_OK;
 }

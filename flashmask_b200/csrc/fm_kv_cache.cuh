@@ -60,6 +60,9 @@ __device__ __forceinline__ uint32_t to_payload2(float lo, float hi) {
   }
 }
 
+// 0x80 in every byte of w that is an e4m3 NaN (0x7f, 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Payload bytes 0, 1 (`lo`) and 2, 3 (`hi`) of a word as pairs of fp16: every payload value is an fp16 value.
 template <bool INT8>
 __device__ __forceinline__ void from_payload4(uint32_t w, uint32_t& lo, uint32_t& hi) {

@@ -300,7 +300,8 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
   cols = std::max<int64_t>(lengths ? cols + S : cols, S);
   const bool bounded = max_seqlen < kNoBound || B * cols * f.Hkv * (f.d + f.dv) * 2 <= kMostDense;
   if (S * (Hq / f.Hkv) > few_rows(f.d, B * f.Hkv) && B > 0 && bounded) {
-    const Tensor shift = fresh({B}, at::kInt, ck), bounds = fresh({B, 1, cols, causal ? 1 : 2}, at::kInt, ck);
+    const Tensor shift = fresh({B}, at::kInt, ck), bounds = fresh({B, 1, cols, causal ? 1 : 2}, at::kInt, ck), marks = fresh({B, f.Hkv}, at::kInt, ck);
+    a.marks = marks.data_ptr<int>();
     check(fm_kv_bounds(&f, &a, (int)cols, shift.data_ptr<int>(), bounds.data_ptr<int>(), stream), "fm_kv_bounds");
     const Tensor k = fresh({B, cols, f.Hkv, f.d}, query.scalar_type(), ck), v = fresh({B, cols, f.Hkv, f.dv}, query.scalar_type(), ck);
     fm_kv_args r = a;
@@ -319,6 +320,8 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
       x.workspace = ws.data_ptr();
     }
     check(fm_fwd(&x, stream), "fm_fwd");
+    a.o = out.data_ptr(); a.lse = lse.data_ptr<float>();
+    check(fm_kv_nan_rows(&f, &a, stream), "fm_kv_nan_rows");
     return {out, lse};
   }
   const Tensor q = vec_rows(query);

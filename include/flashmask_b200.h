@@ -484,6 +484,7 @@ typedef struct fm_kv_args {
   const float* sink;
   void* workspace; size_t workspace_bytes;
   int64_t q_stride[3], k_stride[3], v_stride[3];      /* elements: batch, row, head */
+  int32_t* marks;           /* [B, Hkv] or NULL: see fm_kv_nan_rows                */
 } fm_kv_args;
 
 /* Offset of a position in the payload (elements from k, or from v with `value`), or -1 where the position is no token:
@@ -498,7 +499,8 @@ FM_API int64_t fm_kv_locate(const fm_kv_cache* cache, const fm_kv_args* args, in
 FM_API int fm_kv_write(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
 
 /* k_out [B, S, Hkv, d], v_out [B, S, Hkv, dv] (contiguous): the tokens at positions start[b] + i, zeros where the
- * position is below 0, at seqlens[b] or beyond, or no token.  Exact in bf16; fp16 saturates at 65504. */
+ * position is below 0, at seqlens[b] or beyond, or no token.  Exact in bf16; fp16 saturates at 65504.  With `marks` what
+ * is NaN comes as 0, and marks[b, h] is set where there was some. */
 FM_API int fm_kv_read(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
 
 /* o [B, S, Hq, dv] (contiguous) and lse [B, Hq, S] of q [B, S, Hq, d] against the cache.  Rows i < n = lengths[b] stand
@@ -512,9 +514,15 @@ FM_API int fm_kv_attention(const fm_kv_cache* cache, const fm_kv_args* args, voi
 
 /* For attention with many query rows over tokens read back into dense tensors of `cols` >= S columns: the position of
  * column 0 of every sequence (`shift` [B], the start of an fm_kv_read of `cols` rows) and the column bounds
- * [B, 1, cols, 1 (causal) | 2] with which fm_fwd gives what fm_kv_attention gives. */
+ * [B, 1, cols, 1 (causal) | 2] with which fm_fwd sees what fm_kv_attention sees.  With `marks` those are zeroed. */
 FM_API int fm_kv_bounds(const fm_kv_cache* cache, const fm_kv_args* args, int cols, int32_t* shift, int32_t* bounds,
                         void* stream);
+
+/* After that fm_fwd: NaN in o and lse for the rows that see a NaN key or value, as fm_kv_attention gives it.  A row that
+ * does not see the token must not get it, but the products of a dense forward would hand it on (0 * NaN), so one `marks`
+ * goes through fm_kv_bounds, fm_kv_read and this call.  A NaN key, or a page whose scale is NaN, takes the whole row; a NaN
+ * value in e4m3 its column. */
+FM_API int fm_kv_nan_rows(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -151,3 +151,17 @@ def test_the_oracle_rounds_as_the_type_does():
     assert torch.equal(ref.grid(x, torch.float8_e4m3fn), x.float().to(torch.float8_e4m3fn).double())
     assert ref.least_exponent(448.0, torch.float8_e4m3fn) == 0 and ref.least_exponent(448.5, torch.float8_e4m3fn) == 1
     assert ref.least_exponent(127.0, torch.int8) == 0 and ref.least_exponent(1.0, torch.int8) == -6 and ref.least_exponent(0.0, torch.int8) == -64
+
+
+def test_nan_rows_refusals():
+    lib = _lib.load()
+    table = np.zeros((1, 3), dtype=np.int32)
+    for change, status in ((dict(Hq=3), 1), (dict(window=-1), 1), (dict(window=4, causal=0), 1), (dict(o=None), 1), (dict(lse=None), 1), (dict(seqlens=None), 1),
+                           (dict(marks=None), 1), (dict(dtype=7), 1), (dict(B=-1), 1)):
+        a = args(table)
+        a.marks = 256
+        for key, value in change.items():
+            setattr(a, key, value)
+        assert lib.fm_kv_nan_rows(C.byref(cache()), C.byref(a), None) == status, change
+    for B, S in ((0, 1), (1, 0)):
+        assert lib.fm_kv_nan_rows(C.byref(cache()), C.byref(args(table, B=B, S=S)), None) == 0

@@ -1,0 +1,151 @@
+"""Attention over the cache on both of its paths, the kernel that reads pages and the dense forward over tokens read back, where a
+call can go wrong: NaN that a row does not see, windows and page tables of any width, many K tiles under a mask, wide heads."""
+import math
+
+import pytest
+import torch
+
+import flashmask_b200 as fm
+import _cache_util as ref
+from test_gpu_cache import E4M3, INT8, Filled, rand_q
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+def defined(q, k, v, there, n_rows, causal, window, scale, sink):
+    """One sequence in 64 bits: out [S, Hq, dv], lse [Hq, S], and for the tolerances sum_j p_j |v_j| and the largest sum_c |q_c k_c| of a
+    visible key [S, Hq].  NaN in a key or value reaches the rows that see it."""
+    S, Hq, d = q.shape
+    L, H = k.shape[:2]
+    at = (torch.arange(S, device="cuda") + L - n_rows)[:, None]
+    pos = torch.arange(L, device="cuda")[None]
+    seen = there[None] & ((pos <= at) if causal else torch.ones_like(pos <= at)) & (torch.arange(S, device="cuda") < n_rows)[:, None]
+    if window:
+        seen = seen & (pos > at - window)
+    out, weight = (torch.zeros(S, Hq, v.shape[2], dtype=torch.float64, device="cuda") for _ in range(2))
+    lse, reach = torch.full((Hq, S), -math.inf, dtype=torch.float64, device="cuda"), torch.zeros(S, Hq, dtype=torch.float64, device="cuda")
+    some = seen.any(1)
+    for h in range(Hq):
+        kk, vv = k[:, h * H // Hq], v[:, h * H // Hq]
+        x = torch.where(seen, q[:, h] @ kk.T * scale, torch.full((), -math.inf, dtype=torch.float64, device="cuda"))
+        if sink is not None:
+            x = torch.cat([x, sink[h].double().cuda().expand(S, 1)], 1)
+        lse[h] = torch.logsumexp(x, 1)
+        p = torch.where(seen, torch.softmax(x, 1)[:, :L], torch.zeros((), dtype=torch.float64, device="cuda"))
+        out[:, h] = p @ vv.nan_to_num(nan=0.0)
+        out[:, h][(seen.double() @ vv.isnan().double()) > 0] = math.nan
+        out[~some, h] = 0.0
+        weight[:, h] = p @ vv.abs().nan_to_num(nan=0.0)
+        reach[:, h] = torch.where(seen, q[:, h].abs() @ kk.abs().T, torch.zeros((), dtype=torch.float64, device="cuda")).amax(1) * abs(scale) if L else 0.0
+    return [t.cpu() for t in (out, lse, weight, reach)]
+
+
+def agrees(f, q, pages, *, q_lengths=None, causal=True, window=None, scale=None, sink=None, **kw):
+    """The call against the definition.  `pages`: the kernel that reads pages takes it (p in fp16), else the dense forward (p in
+    q's type).  Where the definition has NaN the result has, and nowhere else; its lse is NaN where a whole row is.
+
+    Half a step of p is 2^-11 in fp16 and 2^-8 in bf16; in fp16 it is absolute below 2^-14: 2^-25, when the largest p is 2^7 at
+    least (pages) or 1 (dense), of values of at most 448 scales.  A score is off by d + 16 steps of 2^-23 of the sum of its
+    products' magnitudes, a sum over n keys by n steps of 2^-24, and the result is rounded once."""
+    B, S, Hq, d = q.shape
+    got = fm.kv_cache_attention(q.cuda(), f.cache, f.table.cuda(), f.seqlens.cuda(), causal=causal, window_size=window,
+                                q_lengths=None if q_lengths is None else i32(q_lengths), softmax_scale=scale,
+                                sink=None if sink is None else sink.cuda(), return_lse=True, **kw)
+    out, lse = got[0].cpu().double(), got[1].cpu().double()
+    half = torch.finfo(q.dtype).eps / 2
+    p_half, p_least = (2.0 ** -11, 2.0 ** -32) if pages else ((2.0 ** -11, 2.0 ** -25) if q.dtype == FP16 else (2.0 ** -8, 0.0))
+    for b in range(B):
+        n = min(max(f.lens[b], 0), f.table.shape[1] * f.page)
+        (k, there), (v, _) = f.dense(b, "k", n), f.dense(b, "v", n)
+        rows = S if q_lengths is None else min(max(q_lengths[b], 0), S)
+        o, l, weight, reach = defined(q[b].double().cuda(), k.cuda(), v.cuda(), there.cuda(), rows, causal, window, 1 / math.sqrt(d) if scale is None else scale, sink)
+        assert torch.equal(torch.isnan(out[b]), torch.isnan(o)), b
+        dead = torch.isnan(o).all(-1)
+        assert torch.equal(torch.isnan(lse[b]), dead.T), b
+        slack = reach * (d + 16) * 2.0 ** -23 + 2.0 ** -20 + max(n, 1) * 2.0 ** -24
+        tol = half * o.abs() + n * p_least * 448 * f.largest_scale(b) + weight * (p_half + 2 * slack[..., None]) + torch.finfo(q.dtype).smallest_normal * half
+        far = ((out[b] - o).abs() - tol).nan_to_num(nan=-1.0)
+        w = far.argmax()
+        assert far.flatten()[w] <= 0, (b, int(w), *(t.flatten()[w].item() for t in (far, out[b], o, weight)))
+        fin = torch.isfinite(l) & ~dead.T
+        assert torch.equal(torch.isinf(lse[b]) | dead.T, ~fin), b
+        ltol = (slack.T + 2.0 ** -21 * l.abs())[fin] + 2.0 ** -20
+        assert ((lse[b] - l).abs()[fin] <= ltol).all(), (b, (lse[b] - l).abs()[fin].max())
+    return got
+
+
+def page_at(f, b, pos):
+    return int(f.table[b, pos // f.page])
+
+
+def plant(f, S):
+    """NaN in a value in the middle of the queries' own tokens (head 0), in a key near the end and in a value at the start (last head).  In int8
+    it is the page's scale that says so, and the whole page that is none."""
+    last = f.cache.k.shape[1] - 1
+    for b, n in enumerate(f.lens):
+        for name, pos, h, dim in (("v", n - S // 2, 0, 7), ("k", n - 3, last, 5), ("v", 3, last, 1)):
+            if pos < 0:
+                continue
+            page = page_at(f, b, pos)
+            if f.kind == E4M3:
+                getattr(f.cache, name).view(torch.uint8)[page, h, pos % f.page, dim] = 0xff if dim == 7 else 0x7f
+            else:
+                getattr(f.cache, name + "_scale")[page, h] = math.nan
+
+
+MASKS = [(True, None, False), (True, 33, True), (False, None, True)]
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+@pytest.mark.parametrize("causal,window,padded", MASKS)
+@pytest.mark.parametrize("S,G,d,dv,dtype,pages", [(20, 4, 128, 128, BF16, True), (40, 4, 128, 128, BF16, False), (40, 3, 64, 64, FP16, False), (120, 1, 80, 48, BF16, False),
+                                                  (40, 4, 192, 128, BF16, True), (40, 4, 256, 256, BF16, False), (20, 4, 256, 256, FP16, True)])
+def test_nan_reaches_the_rows_that_see_it_alone(kind, causal, window, padded, S, G, d, dv, dtype, pages):
+    f = Filled([300, 37, 170], 2, d, dv, kind, 16, seed=31, dtype=dtype)
+    plant(f, S)
+    agrees(f, rand_q(3, S, 2 * G, d, seed=32, dtype=dtype), pages, causal=causal, window=window, q_lengths=[S, 11, S - 9] if padded else None)
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+@pytest.mark.parametrize("S,G,d,dv,dtype", [(32, 4, 64, 64, FP16), (100, 4, 128, 128, BF16), (230, 4, 192, 128, BF16), (300, 2, 128, 64, FP16)])
+def test_nan_in_a_long_prompt_in_parts(kind, S, G, d, dv, dtype):
+    """Many K tiles, dealt to several CTAs; queries of several row blocks; a sink; NaN queries of rows that see something."""
+    f = Filled([2900, 500, 1000], 2, d, dv, kind, 64, seed=33, dtype=dtype)
+    plant(f, S)
+    q = rand_q(3, S, 2 * G, d, seed=34, dtype=dtype)
+    agrees(f, q, False, sink=torch.linspace(-1, 2, 2 * G))
+    agrees(f, q, False, window=700)
+    clean = Filled([2900, 500, 1000], 2, d, dv, kind, 64, seed=33, dtype=dtype)
+    q[1, 5, 1, 3] = math.nan
+    agrees(clean, q, False)
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+def test_many_rows_that_see_no_nan_keep_their_bits(kind):
+    """Slots behind the sequences, pages of others, tokens in front of the window, tokens that only later rows see."""
+    S = 40
+    f, g = (Filled([300, 45], 2, 64, 64, kind, 16, seed=35) for _ in range(2))
+    q = rand_q(2, S, 8, 64, seed=36)
+    nan = 0x7f if kind == E4M3 else 0x80
+    owned = set(f.table.flatten().tolist())
+    for name in "kv":
+        raw = getattr(g.cache, name).view(torch.uint8)
+        for b in range(2):
+            raw[page_at(g, b, g.lens[b]), :, g.lens[b] % 16:] = nan
+        for p in set(range(raw.shape[0])) - owned:
+            raw[p] = nan
+            getattr(g.cache, name + "_scale")[p] = math.nan
+        getattr(g.cache, name + "_scale")[page_at(g, 0, 200)] = math.nan              # positions 192 .. 207: in front of the window
+    a, b = (agrees(x, q, False, window=30) for x in (f, g))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    if kind == E4M3:
+        g.cache.v.view(torch.uint8)[page_at(g, 0, 290), 1, 290 % 16, 9] = 0xff
+        c = agrees(g, q, False, window=30)
+        seen = torch.zeros(2, S, 8, 64, dtype=torch.bool)
+        seen[0, 30:, 4:, 9] = True                                                  # rows from position 290 on, whose windows hold it
+        assert torch.equal(torch.isnan(c[0]).cpu(), seen) and torch.equal(c[0][~seen.cuda()], a[0][~seen.cuda()]) and torch.equal(c[1], a[1])
