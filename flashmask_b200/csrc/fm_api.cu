@@ -45,6 +45,7 @@ int bwd_mma_launch(const AttnKParams& p, int dtype, cudaStream_t s);
 int bwd_preprocess_launch(const AttnKParams& p, int dtype, cudaStream_t s);
 int bwd_dsink_launch(const AttnKParams& p, cudaStream_t s);
 int fwd_sm100_launch(const AttnKParams& p, const fm_attn_args* a, cudaStream_t s);
+int fwd_sm100_max_keys();
 size_t fwd_sm100_workspace_bytes(const fm_attn_args* a);
 int bwd_sm100_launch(const AttnKParams& p, const fm_attn_args* a, cudaStream_t s);
 int bwd_sm100_persist_launch(const AttnKParams& p, const fm_attn_args* a, cudaStream_t s);
@@ -290,6 +291,13 @@ extern "C" int fm_fwd_tile_shape(int d, int dv, int* tile_m, int* tile_n) {
   int rc = fwd_mma_tile_shape(d, dv, tile_m, tile_n);
   if (rc != FM_OK) set_error("fm_fwd_tile_shape: unsupported head dims (d=%d, dv=%d)", d, dv);
   return rc;
+}
+
+// (256 and the wider heads have the warp-MMA kernels for more)
+extern "C" int fm_fwd_max_keys(int d, int dv) {
+  int tm, tn;
+  if (fm_fwd_tile_shape(d, dv, &tm, &tn) != FM_OK) return 0;
+  return fwd_uses_sm100(d, dv) && !pair_dims(d, dv) ? fwd_sm100_max_keys() : INT_MAX;
 }
 
 extern "C" int fm_bwd_tile_shape(int d, int dv, int* tile_m, int* tile_n) {

@@ -789,6 +789,8 @@ static FwdSplitPlan fwd_split_plan(const fm_attn_args* a) {
 
 size_t fwd_sm100_workspace_bytes(const fm_attn_args* a) { return fwd_split_plan(a).bytes; }
 
+int fwd_sm100_max_keys() { return FwdSm100Cfg<128, 128>::LIST_MAX * 128; }      // (the same in every variant)
+
 template <int D, int DV, bool IS_BF16, int BLOCK_SCORE, bool BLOCK_BOS, bool SPLIT = false>
 static int launch_fwd_sm100(const AttnKParams& p, const fm_attn_args* a, cudaStream_t s) {
   using Cfg = FwdSm100Cfg<D, DV>;

@@ -298,8 +298,8 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
   // columns of the dense tensors (with rows that do not count the real ones stand up to S columns further left)
   int64_t cols = std::min<int64_t>(max_seqlen, (int64_t)a.max_pages * f.page_size);
   cols = std::max<int64_t>(lengths ? cols + S : cols, S);
-  const bool bounded = max_seqlen < kNoBound || B * cols * f.Hkv * (f.d + f.dv) * 2 <= kMostDense;
-  if (S * (Hq / f.Hkv) > few_rows(f.d, B * f.Hkv) && B > 0 && bounded) {
+  const bool dense = cols <= fm_fwd_max_keys(f.d, f.dv) && (max_seqlen < kNoBound || B * cols * f.Hkv * (f.d + f.dv) * 2 <= kMostDense);
+  if (S * (Hq / f.Hkv) > few_rows(f.d, B * f.Hkv) && B > 0 && dense) {
     const Tensor shift = fresh({B}, at::kInt, ck), bounds = fresh({B, 1, cols, causal ? 1 : 2}, at::kInt, ck), marks = fresh({B, f.Hkv}, at::kInt, ck);
     a.marks = marks.data_ptr<int>();
     check(fm_kv_bounds(&f, &a, (int)cols, shift.data_ptr<int>(), bounds.data_ptr<int>(), stream), "fm_kv_bounds");

@@ -174,6 +174,8 @@ typedef struct fm_attn_args {
  * {<=64, <=128, 192/128, 256/256, 512/512, 576/512}
  * (flashmask/cute/ops/_common.py:95-132). */
 FM_API int fm_fwd_tile_shape(int d, int dv, int* tile_m, int* tile_n);
+/* The most keys (Sk) that fm_fwd takes at these head dims; 0 where they are not served. */
+FM_API int fm_fwd_max_keys(int d, int dv);
 FM_API int fm_bwd_tile_shape(int d, int dv, int* tile_m, int* tile_n);
 
 /* The library reads its A/B switches from the environment once, when it is loaded

@@ -165,3 +165,9 @@ def test_nan_rows_refusals():
         assert lib.fm_kv_nan_rows(C.byref(cache()), C.byref(a), None) == status, change
     for B, S in ((0, 1), (1, 0)):
         assert lib.fm_kv_nan_rows(C.byref(cache()), C.byref(args(table, B=B, S=S)), None) == 0
+
+
+def test_the_most_keys_of_a_dense_forward():
+    lib = _lib.load()
+    for d, dv, most in ((64, 64, 262144), (80, 48, 262144), (128, 128, 262144), (192, 128, 262144), (256, 256, 2 ** 31 - 1), (576, 512, 2 ** 31 - 1), (192, 192, 0), (72, 640, 0)):
+        assert lib.fm_fwd_max_keys(d, dv) == most, (d, dv)

@@ -149,3 +149,11 @@ def test_many_rows_that_see_no_nan_keep_their_bits(kind):
         seen = torch.zeros(2, S, 8, 64, dtype=torch.bool)
         seen[0, 30:, 4:, 9] = True                                                  # rows from position 290 on, whose windows hold it
         assert torch.equal(torch.isnan(c[0]).cpu(), seen) and torch.equal(c[0][~seen.cuda()], a[0][~seen.cuda()]) and torch.equal(c[1], a[1])
+
+
+@pytest.mark.parametrize("d,dv,S,H", [(64, 64, 40, 2), (128, 128, 40, 1), (192, 128, 340, 2)])
+@pytest.mark.parametrize("bound", [None, 300000])
+def test_more_positions_than_the_dense_forward_takes(d, dv, S, H, bound):
+    """A page table, or an upper bound, of 300000 positions over short sequences: 262144 are the most that the dense forward takes."""
+    f = Filled([400, 37], H, d, dv, E4M3, 128, seed=37, table_pages=2344)
+    agrees(f, rand_q(2, S, 4 * H, d, seed=38), True, max_seqlen=bound)
