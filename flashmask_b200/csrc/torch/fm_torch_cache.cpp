@@ -295,9 +295,11 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
   a.softmax_scale = (float)scale;
   void* stream = stream_of(ck);
   const Tensor sink32 = sink ? sink_fp32(*sink, query) : Tensor();
-  // columns of the dense tensors (with rows that do not count the real ones stand up to S columns further left)
+  // columns of the dense tensors (with rows that do not count the real ones stand up to S columns further left).  The last is the last
+  // row's own position, so a window leaves S + window - 1 that a row can see: FM_FWD_MASK_DENSE holds with any window.
   int64_t cols = std::min<int64_t>(max_seqlen, (int64_t)a.max_pages * f.page_size);
   cols = std::max<int64_t>(lengths ? cols + S : cols, S);
+  if (window > 0) cols = std::min(cols, S + std::min<int64_t>(window, INT_MAX) - 1);
   const bool dense = cols <= fm_fwd_max_keys(f.d, f.dv) && (max_seqlen < kNoBound || B * cols * f.Hkv * (f.d + f.dv) * 2 <= kMostDense);
   if (S * (Hq / f.Hkv) > few_rows(f.d, B * f.Hkv) && B > 0 && dense) {
     const Tensor shift = fresh({B}, at::kInt, ck), bounds = fresh({B, 1, cols, causal ? 1 : 2}, at::kInt, ck), marks = fresh({B, f.Hkv}, at::kInt, ck);

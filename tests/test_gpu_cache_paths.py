@@ -157,3 +157,27 @@ def test_more_positions_than_the_dense_forward_takes(d, dv, S, H, bound):
     """A page table, or an upper bound, of 300000 positions over short sequences: 262144 are the most that the dense forward takes."""
     f = Filled([400, 37], H, d, dv, E4M3, 128, seed=37, table_pages=2344)
     agrees(f, rand_q(2, S, 4 * H, d, seed=38), True, max_seqlen=bound)
+
+
+@pytest.mark.parametrize("window", [1, 64, 1000])
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_window_bounds_what_is_read_back(window, padded):
+    """A window far below the length, with and without an upper bound; a page table whose dense tensors would take 2 GiB without a
+    window takes a few MiB."""
+    f = Filled([5000, 37, 1200], 2, 64, 64, E4M3, 64, seed=39, table_pages=4096)
+    q = rand_q(3, 40, 8, 64, seed=40)
+    kw = dict(window=window, q_lengths=[40, 11, 25] if padded else None)
+    a = agrees(f, q, False, **kw)
+    b = agrees(f, q, False, max_seqlen=5000, **kw)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    args = (q.cuda(), f.cache, f.table.cuda(), f.seqlens.cuda())
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    fm.kv_cache_attention(*args, window_size=window)
+    # the dense tensors: 1039 columns of 3 sequences, 2 heads, 64 + 64 values of 2 bytes, 1.6 MB; out, lse, bounds and partial results beside them
+    assert torch.cuda.max_memory_allocated() - before < 16 << 20
+    # more tokens than the dense forward takes, of which the window leaves few
+    g = Filled([5000, 37, 1200], 2, 64, 64, E4M3, 64, seed=39, table_pages=5000)
+    c = agrees(g, q, False, **kw)
+    assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
