@@ -37,6 +37,10 @@ Tensor vec_rows(const Tensor& t) {
 // (a dimension of one element may carry any stride)
 void vec_strides(int64_t* out, const Tensor& t) { for (int i = 0; i < 3; ++i) out[i] = t.size(i) == 1 ? 0 : t.stride(i); }
 
+// Whether a forward-mode derivative comes with t: requires_grad and GradMode say nothing of it.
+bool has_tangent(const Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined(); }
+bool has_tangent(const std::optional<Tensor>& t) { return t && has_tangent(*t); }
+
 Tensor packed(const Tensor& t) {
   const Tensor c = t.contiguous();
   return c.numel() == 0 || aligned16(c) ? c : c.clone();
@@ -146,7 +150,7 @@ std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const st
   const int64_t d = q.size(3);
   require(cos.dim() == 2 && cos.sizes() == sin.sizes() && 2 * cos.size(1) <= d, "cos and sin must be [positions, n] with 2 n <= head dim");
   require(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "cos and sin must be float32");
-  require(!cos.requires_grad() && !sin.requires_grad(), "cos and sin take no gradient");
+  require(!cos.requires_grad() && !sin.requires_grad() && !has_tangent(cos) && !has_tangent(sin), "cos and sin take no gradient");
   for (const auto* w : {&qw, &kw}) {
     if (!*w) continue;
     require((*w)->dim() == 1 && (*w)->size(0) == d, "weights must be [head dim]");
@@ -161,6 +165,7 @@ std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const st
             (pos->dim() == 2 && pos->size(1) == q.size(1) && (pos->size(0) == q.size(0) || pos->size(0) == 1)), "positions must be [B, S] or [S]");
   }
   pybind11::gil_scoped_release nogil;
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(q) || has_tangent(k) || has_tangent(qw) || has_tangent(kw)), "qk_norm_rotary has no forward-mode derivative");
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || (qw && qw->requires_grad()) || (kw && kw->requires_grad())))
     return norm_forward(q, k, qw, kw, cos, sin, pos, eps, interleaved, nullptr);
   const variable_list r = NormRotary::apply(q, k, qw, kw, cos, sin, pos, eps, interleaved);
@@ -168,10 +173,16 @@ std::pair<Tensor, Tensor> norm_rotary(const Tensor& q, const Tensor& k, const st
 }
 
 // ---------------------------------------------------------------------------- cache
+void no_gradient(const Tensor& t, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no gradient: call it under torch.no_grad()");
+  TORCH_CHECK(!has_tangent(t), what, " has no gradient, and none in forward mode");
+}
+
 struct Cache { const Tensor &k, &v, &ks, &vs; };
 
-fm_kv_cache cache_of(const Cache& c) {
+fm_kv_cache cache_of(const Cache& c, const char* what) {
   fm_kv_cache r;
+  for (const Tensor* t : {&c.k, &c.v, &c.ks, &c.vs}) no_gradient(*t, what);
   require(c.k.dim() == 4 && c.v.dim() == 4 && c.k.sizes().slice(0, 3) == c.v.sizes().slice(0, 3),
           "cache k and v must be [num_pages, Hkv, page_size, D]");
   require(c.k.scalar_type() == c.v.scalar_type() && (c.k.scalar_type() == at::kFloat8_e4m3fn || c.k.scalar_type() == at::kChar),
@@ -209,15 +220,11 @@ fm_kv_args kv_args(const Cache& c, const Tensor& table, int64_t B, int64_t S, Te
   return a;
 }
 
-void no_gradient(const Tensor& t, const char* what) {
-  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, " has no gradient: call it under torch.no_grad()");
-}
-
 void kv_write(const Tensor& ck, const Tensor& cv, const Tensor& cks, const Tensor& cvs, const Tensor& key_in, const Tensor& value_in,
               const Tensor& table, const Tensor& start, const std::optional<Tensor>& lengths) {
   const Cache c{ck, cv, cks, cvs};
   TORCH_CHECK(ck.is_cuda() && key_in.is_cuda(), kNoCpu);
-  const fm_kv_cache f = cache_of(c);
+  const fm_kv_cache f = cache_of(c, "kv_cache_write");
   require(key_in.dim() == 4 && value_in.dim() == 4 && key_in.sizes().slice(0, 3) == value_in.sizes().slice(0, 3) && key_in.size(2) == f.Hkv &&
           key_in.size(3) == f.d && value_in.size(3) == f.dv, "key and value must be [B, S, Hkv, D] of the cache's heads");
   require(key_in.scalar_type() == value_in.scalar_type(), "key and value must share a dtype");
@@ -240,7 +247,7 @@ std::pair<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Tens
                                   const Tensor& start, const Tensor& seqlens, int64_t length, at::ScalarType dtype) {
   const Cache c{ck, cv, cks, cvs};
   TORCH_CHECK(ck.is_cuda(), kNoCpu);
-  const fm_kv_cache f = cache_of(c);
+  const fm_kv_cache f = cache_of(c, "kv_cache_read");
   require(length >= 0, "length must not be negative");
   const c10::cuda::CUDAGuard guard(ck.device());
   Tensor keep[3];
@@ -273,7 +280,7 @@ std::pair<Tensor, Tensor> kv_attention(const Tensor& query, const Tensor& ck, co
                                        int64_t max_seqlen) {
   const Cache c{ck, cv, cks, cvs};
   TORCH_CHECK(ck.is_cuda() && query.is_cuda(), kNoCpu);
-  const fm_kv_cache f = cache_of(c);
+  const fm_kv_cache f = cache_of(c, "kv_cache_attention");
   require(query.dim() == 4 && query.size(3) == f.d, "query must be [B, S, H, D] of the cache's head dim");
   require(f.Hkv > 0 && query.size(2) % f.Hkv == 0 && query.size(2) > 0, "num q heads must be a multiple of num kv heads");
   require(query.device() == ck.device(), "query must be on the cache's device");

@@ -26,5 +26,6 @@ def qk_norm_rotary(query: torch.Tensor, key: torch.Tensor, q_weight: Optional[to
     stand, e.g. from 0 in every packed document; without it token i stands at i.  A position that the tables do not have makes its rows
     NaN.  Sums and products are fp32, rounded once.
 
-    Gradients of query, key and the weights are exact to the same rounding and bitwise reproducible; they have no gradients themselves."""
+    Gradients of query, key and the weights are exact to the same rounding and bitwise reproducible; they have no gradients themselves.
+    There is no forward-mode derivative: dual tensors are refused."""
     return _native_host().norm_rotary(query, key, q_weight, k_weight, cos, sin, positions, eps, interleaved)

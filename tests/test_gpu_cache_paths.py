@@ -181,3 +181,36 @@ def test_a_window_bounds_what_is_read_back(window, padded):
     g = Filled([5000, 37, 1200], 2, 64, 64, E4M3, 64, seed=39, table_pages=5000)
     c = agrees(g, q, False, **kw)
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+def test_tangents_are_refused():
+    """No operator of the cache has a derivative: a dual tensor is refused, under no_grad too, and not taken for a constant."""
+    import torch.autograd.forward_ad as ad
+    f = Filled([20], 2, 64, 64, E4M3, 16, seed=50)
+    q, t, n = rand_q(1, 1, 4, 64).cuda(), f.table.cuda(), f.seqlens.cuda()
+    k = torch.ones(1, 1, 2, 64, dtype=BF16, device="cuda")
+    sink = torch.zeros(4, device="cuda")
+    with ad.dual_level():
+        dual = lambda x: ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: fm.kv_cache_attention(dual(q), f.cache, t, n), lambda: fm.kv_cache_attention(q, f.cache, t, n, sink=dual(sink)),
+                     lambda: fm.kv_cache_write(f.cache, dual(k), k, t, n), lambda: fm.kv_cache_write(f.cache, k, dual(k), t, n)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        fm.kv_cache_attention(q, f.cache, t, n, sink=sink)
+
+
+def test_caches_that_want_a_gradient_are_refused():
+    f = Filled([20], 2, 64, 64, E4M3, 16, seed=51)
+    t, n = f.table.cuda(), f.seqlens.cuda()
+    k = torch.ones(1, 1, 2, 64, dtype=BF16, device="cuda")
+    for name in ("k_scale", "v_scale"):
+        getattr(f.cache, name).requires_grad_(True)
+        for call in (lambda: fm.kv_cache_attention(rand_q(1, 1, 4, 64).cuda(), f.cache, t, n), lambda: fm.kv_cache_read(f.cache, t, n - 5, n, 5),
+                     lambda: fm.kv_cache_write(f.cache, k, k, t, n)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad():
+                call()
+        getattr(f.cache, name).requires_grad_(False)

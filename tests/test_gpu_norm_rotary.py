@@ -273,3 +273,18 @@ def test_no_second_derivative():
         assert torch.equal(a, b)
         with pytest.raises(NotImplementedError, match="no gradient"):
             a.float().square().sum().backward(retain_graph=True)
+
+
+def test_tangents_are_refused():
+    """The operator has no forward-mode derivative: a dual tensor is refused, under no_grad too, and not taken for a constant."""
+    import torch.autograd.forward_ad as ad
+    q, k, _, _, w, cos, sin, pos = problem(1, 4, 2, 1, 64, 32, torch.bfloat16, torch.bfloat16, seed=12)
+    args = [q, k, *w, cos, sin]
+    with ad.dual_level():
+        for i in range(6):
+            dual = [ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises((RuntimeError, AssertionError)):
+                fm.qk_norm_rotary(*dual, pos)
+            with torch.no_grad(), pytest.raises((RuntimeError, AssertionError)):
+                fm.qk_norm_rotary(*dual, pos)
+        fm.qk_norm_rotary(*args, pos)
