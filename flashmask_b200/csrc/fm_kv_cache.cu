@@ -130,7 +130,9 @@ __global__ void __launch_bounds__(THREADS, write_threads(INT8, VEC) / THREADS) k
       *to = v;
     }
   }
-  // every thread has read the old scale (it waited for the others' magnitudes), so it can go
+  // Every thread has read the old scale, so it can go: a CTA's barrier lies between, a warp's lanes have only exchanged their
+  // magnitudes, which orders no memory.
+  if constexpr (WARPS == 1) __syncwarp();
   if ((threadIdx.x & (TEAM - 1)) == 0) *scale = INT8 && (bad || old_nan) ? __uint_as_float(0x7fffffffu) : exp2_int(e);
 }
 

@@ -183,6 +183,27 @@ def test_a_window_bounds_what_is_read_back(window, padded):
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
 
 
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+def test_appends_that_grow_the_scale_of_pages_that_warps_take(kind):
+    """A token appended to each of 256 pages of 8 heads, 4096 warps side by side, each token larger than those before: the earlier
+    tokens are rounded again from the scale that the page had."""
+    B, H, d, page = 256, 8, 32, 16
+    cache = fm.QuantizedKVCache.empty(B, H, d, page_size=page, dtype=kind)
+    table = torch.randperm(B, generator=torch.Generator().manual_seed(48)).int()[:, None]
+    vals = {n: getattr(cache, n).cpu().float().double()[:4] for n in "kv"}
+    where = [int((table[:, 0] == p).nonzero()) for p in range(4)]                  # sequences of the pages that the oracle follows
+    sc = {n: getattr(cache, n + "_scale").cpu().double()[:4] for n in "kv"}
+    g = torch.Generator().manual_seed(49)
+    for step in range(6):
+        x = {n: (torch.randn(B, 1, H, d, generator=g) * 3.0 ** step).bfloat16() for n in "kv"}
+        fm.kv_cache_write(cache, x["k"].cuda(), x["v"].cuda(), table.cuda(), i32([step] * B))
+        for n in "kv":
+            ref.write((vals[n], kind), sc[n], x[n][where], torch.arange(4).int()[:, None], [step] * 4, None)
+    for n in "kv":
+        assert torch.equal(getattr(cache, n + "_scale").cpu().double()[:4], sc[n])
+        assert torch.equal(getattr(cache, n).cpu().float().double()[:4], vals[n])
+
+
 def test_tangents_are_refused():
     """No operator of the cache has a derivative: a dual tensor is refused, under no_grad too, and not taken for a constant."""
     import torch.autograd.forward_ad as ad
