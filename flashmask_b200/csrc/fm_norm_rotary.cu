@@ -119,8 +119,8 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// cos and sin of slot s at the token's position: (1, 0) behind the rotated part, NaN where the table does not have the
-// position, so that the mistake shows in the result.
+// cos and sin of slot s at the token's position: (1, 0) behind the rotated part, NaN for the whole row where the table does not
+// have the position, so that the mistake shows in the result.  (Without a rotated part positions say nothing.)
 __device__ __forceinline__ void load_angles(const NormParams& p, int64_t b, int t, int s, bool on, f2 (&c)[4], f2 (&sn)[4]) {
   int64_t pos = t;
   if (p.pos) pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[b * p.pos_b + t] : reinterpret_cast<const int32_t*>(p.pos)[b * p.pos_b + t];
@@ -132,9 +132,10 @@ __device__ __forceinline__ void load_angles(const NormParams& p, int64_t b, int 
     c[0] = c0.x; c[1] = c0.y; c[2] = c1.x; c[3] = c1.y;
     sn[0] = s0.x; sn[1] = s0.y; sn[2] = s1.x; sn[3] = s1.y;
   } else {
+    const bool none = p.rot > 0 && !there;
     const float nan = __uint_as_float(0x7fffffffu);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { c[i] = turned ? pair(nan, nan) : pair(1.f, 1.f); sn[i] = turned ? pair(nan, nan) : pair(0.f, 0.f); }
+    for (int i = 0; i < 4; ++i) { c[i] = none ? pair(nan, nan) : pair(1.f, 1.f); sn[i] = none ? pair(nan, nan) : pair(0.f, 0.f); }
   }
 }
 
@@ -237,8 +238,7 @@ struct NormStream {
     const int64_t pos = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[a.b * p.pos_b + a.t] : reinterpret_cast<const int32_t*>(p.pos)[a.b * p.pos_b + a.t];
     return pos >= 0 && pos < p.table ? (int)pos : -1;
   }
-  // The job's rows from its first group on, and its angles: NaN where the tables do not have the position, so that the
-  // mistake shows in the result.
+  // The job's rows from its first group on, and its angles: as load_angles() gives them.
   __device__ __forceinline__ void begin() {
     if (job >= jobs) return;
     const NormJob a = place(job);
@@ -259,7 +259,8 @@ struct NormStream {
         cp_async16(to + LPR * 32, n, true);
         cp_async16(to + LPR * 48, n + 4, true);
       } else {                                                   // (cos, sin) = (1, 0) behind the rotated part
-        const uint32_t c = turned ? 0x7fffffffu : 0x3f800000u, n = turned ? 0x7fffffffu : 0u;
+        const bool none = p.rot > 0 && pos < 0;
+        const uint32_t c = none ? 0x7fffffffu : 0x3f800000u, n = none ? 0x7fffffffu : 0u;
 #pragma unroll
         for (int i = 0; i < 4; ++i) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(to + LPR * 16 * i), "r"(i < 2 ? c : n) : "memory");
       }

@@ -24,7 +24,7 @@ def qk_norm_rotary(query: torch.Tensor, key: torch.Tensor, q_weight: Optional[to
     with the rows of ``cos`` and ``sin`` (fp32 [positions, n], n a multiple of 8) at the token's position; pairs are
     ``(i, i + n)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.  ``positions`` (int32 / int64, [B, S] or [S]) says where tokens
     stand, e.g. from 0 in every packed document; without it token i stands at i.  A position that the tables do not have makes its rows
-    NaN.  Sums and products are fp32, rounded once.
+    NaN, what does not turn included (with n = 0 positions say nothing).  Sums and products are fp32, rounded once.
 
     Gradients of query, key and the weights are exact to the same rounding and bitwise reproducible; they have no gradients themselves.
     There is no forward-mode derivative: dual tensors are refused."""

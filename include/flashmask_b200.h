@@ -421,7 +421,7 @@ FM_API int fm_bwd_static_scratch(const fm_attn_args* args, void* stream);
 /* For every row x of d values (a head of a token): u = x / sqrt(mean(x^2) + eps) * weight, then the pairs (a, b) of the
  * first `rot` values turn by the angles of the token's position: (a cos - b sin, b cos + a sin).  A pair is
  * (i, i + rot / 2), or (2 i, 2 i + 1) with `interleaved`.  q and k go through one launch.  Sums and products are fp32;
- * results are rounded once.  A position outside of the tables makes its rows NaN.
+ * results are rounded once.  A position outside of the tables makes its rows NaN (with rot = 0 none is looked up).
  * Strides are in elements (batch, token, head), multiples of 8; tensors, weights and tables are 16-byte aligned; the
  * head dim is contiguous, a multiple of 16 up to 512, `rot` a multiple of 16.  No counterpart in the reference, which
  * begins at attention. */

@@ -288,3 +288,26 @@ def test_tangents_are_refused():
             with torch.no_grad(), pytest.raises((RuntimeError, AssertionError)):
                 fm.qk_norm_rotary(*dual, pos)
         fm.qk_norm_rotary(*args, pos)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,n", [(64, 16), (128, 32), (96, 24), (256, 64), (512, 8)])
+def test_a_position_outside_takes_the_whole_row(interleaved, d, n):
+    """NaN in what does not turn as well, and in the gradients of the same rows; the others keep their bits.  Without a
+    rotated part positions say nothing."""
+    cos, sin = tables(10, n)
+    g = torch.Generator().manual_seed(11)
+    x, gy = (torch.randn(1, 5, 3, d, generator=g).bfloat16().cuda() for _ in range(2))
+    pos = torch.tensor([[0, 10, 9, -1, 2 ** 40]], device="cuda")
+    bad = torch.tensor([False, True, False, True, True], device="cuda")
+    runs = []
+    for p in (pos, pos.clamp(0, 9)):
+        leaf, w = x.clone().requires_grad_(True), torch.ones(d, device="cuda").requires_grad_(True)
+        y, _ = fm.qk_norm_rotary(leaf, x, w, None, cos, sin, p, interleaved=interleaved)
+        runs.append((y, *torch.autograd.grad(y, [leaf, w], gy)))
+    for a, b in zip(runs[0][:2], runs[1][:2]):
+        assert torch.isnan(a[:, bad]).all() and torch.equal(a[:, ~bad], b[:, ~bad])
+    assert torch.isnan(runs[0][2]).all()
+    none = torch.zeros(10, 0, device="cuda")
+    y, _ = fm.qk_norm_rotary(x, x, None, None, none, none, pos)
+    assert torch.isfinite(y).all()
