@@ -41,10 +41,11 @@ __global__ void __launch_bounds__(THREADS, write_threads(INT8, VEC) / THREADS) k
   if (THREADS > TEAM && h >= p.g.Hkv) return;
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int start = p.start[b];
-  if (n + min(start, 0) <= 0 || start > INT_MAX - p.S) return;  // (rows before position 0 are not written)
-  const int first = max(start, 0), last = start + n - 1;         // positions
-  const int base = ((first >> p.g.page_log2) + (int)blockIdx.x) << p.g.page_log2;
-  if (base > last || base < 0) return;
+  // positions that are written: none before 0 or behind the page table (2^31 - 2^16 at most), however far the rows reach
+  const int first = max(start, 0), last = (int)min((int64_t)start + n, (int64_t)p.g.cap) - 1;
+  const int64_t base64 = (int64_t)((first >> p.g.page_log2) + blockIdx.x) << p.g.page_log2;
+  if (last < first || base64 > last) return;
+  const int base = (int)base64;
   const int page = kv_page(p.g, p.table + b * p.g.table_stride, base);
   if (page < 0) return;
   const int w = p.width[which];

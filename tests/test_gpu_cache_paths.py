@@ -183,6 +183,24 @@ def test_a_window_bounds_what_is_read_back(window, padded):
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
 
 
+def test_positions_at_the_end_of_a_table_of_two_billion():
+    """A write of 70000 rows, of which five count, that starts near the end of a page table of 2^31 - 2^16 - 128 positions; and one that
+    runs over that end."""
+    page, n = 128, (2 ** 31 - 2 ** 16) // 128 - 1
+    table = torch.full((1, n), -1, dtype=torch.int32, device="cuda")
+    table[0, n - 1], table[0, n - 2] = 1, 0
+    x = torch.randn(1, 70000, 1, 16, generator=torch.Generator().manual_seed(47)).bfloat16().cuda()
+    for start, rows in ((n * page - page - 2, 5), (n * page - 4, 70000)):
+        cache = fm.QuantizedKVCache.empty(2, 1, 16, page_size=page)
+        fm.kv_cache_write(cache, x, x, table, i32([start]), i32([rows]))
+        want = fm.QuantizedKVCache.empty(2, 1, 16, page_size=page)
+        at = start - (n - 2) * page                                                 # the same slots through a table of two pages
+        fm.kv_cache_write(want, x[:, :256].contiguous(), x[:, :256].contiguous(), i32([[0, 1]]), i32([at]), i32([min(rows, 256)]))
+        assert want.k.view(torch.uint8).any()
+        for a in ("k", "v", "k_scale", "v_scale"):
+            assert torch.equal(getattr(cache, a).view(torch.uint8), getattr(want, a).view(torch.uint8)), (a, start)
+
+
 @pytest.mark.parametrize("kind", [E4M3, INT8])
 def test_appends_that_grow_the_scale_of_pages_that_warps_take(kind):
     """A token appended to each of 256 pages of 8 heads, 4096 warps side by side, each token larger than those before: the earlier
