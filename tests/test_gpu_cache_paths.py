@@ -183,6 +183,32 @@ def test_a_window_bounds_what_is_read_back(window, padded):
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
 
 
+@pytest.mark.parametrize("d,dv,dtype", [(64, 64, FP16), (80, 80, BF16), (96, 96, FP16), (96, 128, BF16), (112, 16, BF16), (128, 128, BF16)])
+@pytest.mark.parametrize("S,G,window,causal", [(32, 4, None, True), (100, 1, 700, True), (64, 4, None, False), (40, 3, 2000, True), (300, 4, 1500, True)])
+def test_many_tiles_under_a_mask(d, dv, dtype, S, G, window, causal):
+    """The dense forward's deal of K tiles to CTAs and sub-tiles when a mask tensor is there: parts that lengths and windows leave
+    empty, one row block (sub-tiles in turn) and several, packed heads and not, rows that see nothing."""
+    f = Filled([4100, 37, 700], 2, d, dv, E4M3, 64, seed=41, dtype=dtype)
+    q = rand_q(3, S, 2 * G, d, seed=42, dtype=dtype)
+    agrees(f, q, False, window=window, causal=causal)
+    agrees(f, q, False, window=window, causal=causal, q_lengths=[S, 0, S // 2], sink=torch.linspace(-2, 2, 2 * G))
+
+
+@pytest.mark.parametrize("d,dv,S", [(192, 128, 130), (192, 128, 225), (256, 256, 30)])
+@pytest.mark.parametrize("kind", [E4M3, INT8])
+def test_wide_heads_with_many_rows_keep_the_precision_of_pages(d, dv, S, kind):
+    """Three sequences of two kv heads: up to 900 | 150 rows stay with the kernel that reads pages, whose p is fp16 whatever q is."""
+    f = Filled([300, 37, 150], 2, d, dv, kind, 32, seed=43)
+    agrees(f, rand_q(3, S, 8, d, seed=44), True, q_lengths=[S, 20, S - 9])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_scales_that_turn_scores_round(scale):
+    f = Filled([300, 37], 2, 64, 64, E4M3, 16, seed=45)
+    for S, pages in ((3, True), (40, False)):
+        agrees(f, rand_q(2, S, 8, 64, seed=46), pages, scale=scale, window=50)
+
+
 def test_positions_at_the_end_of_a_table_of_two_billion():
     """A write of 70000 rows, of which five count, that starts near the end of a page table of 2^31 - 2^16 - 128 positions; and one that
     runs over that end."""
