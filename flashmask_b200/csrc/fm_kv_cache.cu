@@ -173,11 +173,6 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
     pay[x] = p.pay[x] + ph * P * p.width[x] + at[x].col * 8;
   }
   bool found = false;
-  if constexpr (MARK) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      if (scale[x] != scale[x]) { scale[x] = 0.f; found = lo < min(hi, valid); }
-  }
   for (int row0 = lo; row0 < hi; row0 += READ_ILP * min(at[0].step, at[1].step)) {
     uint2 v[2][READ_ILP];
     const int upto = min(hi, row0 + READ_ILP * min(at[0].step, at[1].step));
@@ -207,7 +202,10 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const __grid_constant__
         }
         payload_f32<INT8>(v[x][i].x, a);
         payload_f32<INT8>(v[x][i].y, c);
-        const float sc = row < valid ? scale[x] : 0.f;            // (a NaN scale is no token's)
+        float sc = row < valid ? scale[x] : 0.f;                  // (a NaN scale is no token's)
+        if constexpr (MARK) {
+          if (sc != sc) { sc = 0.f; found = true; }               // (looked at here: the payload is asked for before the scale is there)
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           a[j] *= sc; c[j] *= sc;
@@ -277,15 +275,14 @@ __global__ void __launch_bounds__(256) kv_nan_kernel(const __grid_constant__ KvN
   const int b = blockIdx.z, h = blockIdx.y, i0 = blockIdx.x * NAN_ROWS, rows = min(NAN_ROWS, p.S - i0);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dv = p.width[1], words = dv / 4;
   const float nan = __uint_as_float(0x7fffffffu);
-  auto head_row = [&](int x, int& hq, int& i) { hq = h * p.G + x / rows; i = i0 + x % rows; };
   grid_dep_wait();
-  for (int x = tid; x < rows * p.G; x += 256) {
-    int hq, i;
-    head_row(x, hq, i);
-    float* lse = p.lse + ((int64_t)b * p.Hq + hq) * p.S + i;
-    if (__ldcg(lse) == -INFINITY && (__ldcg(p.o + (((int64_t)b * p.S + i) * p.Hq + hq) * dv) & 0x7fffu) > INF) *lse = nan;
-  }
-  if (__ldcg(p.marks + (int64_t)b * p.g.Hkv + h) == 0) return;
+  const int mark = __ldcg(p.marks + (int64_t)b * p.g.Hkv + h);
+  if (lane < rows)
+    for (int hq = h * p.G + warp; hq < (h + 1) * p.G; hq += 8) {
+      float* lse = p.lse + ((int64_t)b * p.Hq + hq) * p.S + i0 + lane;
+      if (__ldcg(lse) == -INFINITY && (__ldcg(p.o + (((int64_t)b * p.S + i0 + lane) * p.Hq + hq) * dv) & 0x7fffu) > INF) *lse = nan;
+    }
+  if (mark == 0) return;
   const int len = kv_len(p.g, p.seqlens[b]), n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int live = min(rows, n - i0);                            // rows that are queries
   if (live <= 0) return;
