@@ -64,14 +64,14 @@ def kv_cache_write(cache: QuantizedKVCache, key: torch.Tensor, value: torch.Tens
     only values that become subnormal).  Slots behind the last token are left as they are.  A NaN or an infinity reads back
     as NaN; in int8 so does the whole page of that head, until the page begins anew.  Magnitudes below about 2^-73 (e4m3) or
     2^-65 (int8) become zero, those near the end of bf16's range saturate.  A page must not be written for two sequences in
-    one call; pages that sequences share are written once and then only read."""
+    one call, nor appear twice in the row that one writes through; pages that sequences share are written once and then only read."""
     _native_host().kv_write(cache.k, cache.v, cache.k_scale, cache.v_scale, key, value, page_table, start, lengths)
 
 
 def kv_cache_read(cache: QuantizedKVCache, page_table: torch.Tensor, start: torch.Tensor, seqlens: torch.Tensor, length: int, *,
                   dtype: torch.dtype = torch.bfloat16):
     """(key [B, length, Hkv, d], value [B, length, Hkv, dv]): the tokens at positions ``start[b] + i``; zeros where that is
-    negative or not below ``seqlens[b]``.  Exact in bf16; in fp16 magnitudes beyond 65504 saturate."""
+    negative or not below ``seqlens[b]``.  Exact in bf16; in fp16 magnitudes beyond 65504 saturate, and below 2^-14 they are rounded to multiples of 2^-24."""
     if dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"kv_cache_read gives bfloat16 / float16, got {dtype}")
     return _native_host().kv_read(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, start, seqlens, length,
@@ -98,7 +98,11 @@ def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, page_table:
     with lengths that change between replays.  With more rows the tokens are read back into 16-bit tensors of ``max_seqlen`` positions
     (an upper bound of ``seqlens``; without it the
     whole page table, as long as that takes no more than 2 GiB), with a window no more than its last S + ``window_size`` - 1, and go through the dense forward; more positions than it takes (262144 at
-    head dims other than 256) stay with the pages.  At most 1024 sequences."""
+    head dims other than 256) stay with the pages.  At most 1024 sequences where the pages are read as they are.
+
+    Precision: sums and statistics are fp32.  Where the pages are read as they are, the weights p are rounded to fp16 (half a step is 2^-11) whatever query's
+    type, and keys and values are exact; the dense forward rounds p to query's type (2^-8 in bf16) and takes the tokens as ``kv_cache_read`` gives them in
+    that type, so with fp16 queries values of a cache that was written in bf16 saturate and lose small magnitudes as they do there."""
     if sink is not None and learnable_sink is not None:
         raise ValueError("pass either sink or learnable_sink, not both")
     if window_size is not None and window_size < 1:

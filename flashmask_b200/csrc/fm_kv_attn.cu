@@ -23,8 +23,8 @@
 //
 // Bound by HBM, (d + dv) bytes a key, once a call is long: 8 x 32768 keys, 32 / 8 heads, d = 128, one token: 88 us, 6.1
 // TB/s; 8 x 8192: 30 us, 4.5 TB/s (of which 4 us until the first data are there, 4 us behind the last, and CTAs that end between 20 and
-// 26 us: memory serves them unevenly); 64 x 4096, d = 64, int8: 54 us, 4.9 TB/s.  From 16 rows on the dependent instructions of too few
-// warps bind, 8 x 8192 with 16 rows 35 us and 32 rows 50 us: 255 registers leave two CTAs to an SM.
+// 26 us: memory serves them unevenly); 64 x 4096, d = 64, int8: 55 us, 4.9 TB/s.  From 16 rows on the dependent instructions of too few
+// warps bind, 8 x 8192 with 16 rows 36 us and 32 rows 51 us: 255 registers (with 32 rows, d = 128, e4m3 136 bytes of spills besides) leave two CTAs to an SM.
 #include <algorithm>
 
 #include "fm_kv_cache.cuh"

@@ -30,8 +30,10 @@ __device__ __forceinline__ RowWalk row_walk(int upr) {
 // A page that held tokens before (the write starts inside it) keeps its scale or grows it; where it grows, the payload
 // of the earlier tokens is rounded on the new grid.  Slots behind the last new token are left as they are.
 // VEC = units of 8 values that a thread holds.
-// Threads on an SM.  64 registers for eight units spill less in int8 than in e4m3: 2 x 8192 tokens, 8 heads, d = 128, pages of 64 with
-// 1024 / 896 threads: int8 20.9 / 22.0 us, e4m3 23.3 / 19.3 us.
+// Threads on an SM.  At these limits the CTAs' variants spill 60 to 196 bytes, and fewer threads with fewer spills take longer: pages of 64,
+// us with these and with 1024 | 768 | 256 threads for 4 | 8 | 16 units: 4 x 8192 tokens, 8 heads, d = 64 (4 units) e4m3 20.8 / 26.1, int8 23.3 / 24.9; 2 x 8192,
+// d = 128 (8 units) 19.2 / 19.7, 20.4 / 22.3; 4 heads, d = 256, pages of 128 (16 units) 25.8 / 32.5, 26.7 / 36.9.  64 registers for eight units spill less in
+// int8 than in e4m3: with 1024 / 896 threads int8 20.9 / 22.0, e4m3 23.3 / 19.3.
 constexpr int write_threads(bool int8, int vec) { return vec <= 4 ? 1280 : (vec > 8 ? 512 : (int8 ? 1024 : 896)); }
 template <bool IS_BF16, bool INT8, int VEC, int THREADS, int TEAM>
 __global__ void __launch_bounds__(THREADS, write_threads(INT8, VEC) / THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p) {
@@ -149,7 +151,8 @@ struct KvReadParams {
 
 // dst[b, i, h, :] = the token at position start[b] + i, zeros where it has none.  One team (a CTA, or each of its warps) = the rows in one page of one kv
 // head, K and V: the page and its scales are looked up once, and a thread has READ_ILP units of 8 bytes of each in flight.
-// Bound by HBM: 3 bytes a value (2 x 8192 tokens of 8 heads, d = 128, 100 MB: 16 us, 6.3 TB/s; CTAs of 256 threads 18.5 us).
+// Bound by HBM: 3 bytes a value (2 x 8192 tokens of 8 heads, d = 128, 100 MB: e4m3 14.5 us, int8 16, 6.3 TB/s; CTAs of 256 threads 18.5 us).
+// Eight CTAs to an SM at 64 registers and up to 20 bytes of spills; seven: e4m3 14.9, int8 15.6.
 // MARK: for a dense forward, whose P V would take 0 * NaN into rows that do not see the token.  What is NaN comes as 0, and
 // marks[b, h] says that there was some; kv_nan_kernel brings it to the rows that see it.
 constexpr int READ_ILP = 4;
@@ -255,8 +258,8 @@ __global__ void __launch_bounds__(256) kv_bounds_kernel(const KvBoundsParams p) 
 // NaN for the rows of a dense forward that see a token whose key or value is none (it got 0 in its place): the whole row and its
 // lse where a key or a page's scale is NaN, the value's column where a value in e4m3 is.  And an lse of NaN for the other rows
 // of NaN, those of a NaN query, which the dense forward leaves with -inf.
-// One CTA = up to NAN_ROWS query rows of a sequence and kv head.  Nearly always there is no mark, and a CTA reads its rows' lse and leaves (512
-// rows, 32 / 8 heads: 128 CTAs, one round trip to memory).  With a mark its warps walk the groups of 16 tokens that one of the rows sees, lanes
+// One CTA = up to NAN_ROWS query rows of a sequence and kv head.  Nearly always there is no mark, and a CTA reads its rows' lse and leaves:
+// the launch and one round trip to memory (512 rows of 16384 tokens, 32 / 8 heads: 160 -> 164 us; 40 of 300: 17.6 -> 19.5; 64 sequences, 25 of 512: 96 -> 102).  With a mark its warps walk the groups of 16 tokens that one of the rows sees, lanes
 // side by side along the payload; tokens that all rows see, nearly all, cost no work per row.
 struct KvNanParams {
   KvGeom g;

@@ -147,8 +147,9 @@ __device__ __forceinline__ NormJob norm_job(const NormParams& p, int which, int 
 }
 
 // Forward.  A warp has one job, and the rows of the next two groups are on their way while one is worked on: 2 x 8192 tokens,
-// 32 / 8 heads, d = 128, bf16 (335 MB) in 59 us, 5.7 TB/s; with the backward's stream through shared memory 70 us.  80
-// registers: six CTAs of 128 threads to an SM; at 72 the spills cost more than the seventh brings (64 us).
+// 32 / 8 heads, d = 128, bf16 (335 MB) in 66 us, 5.1 TB/s, one call behind the other (alone 60: a part of what is written stays in L2); with
+// the backward's stream through shared memory alone 70 us.  80 registers: six CTAs of 128 threads to an SM, at 20 to 36 bytes of spills; five
+// without any 66 us (4 x 4096 tokens, 16 / 4 heads, d = 64: 26.8 with six, 25.5 with five); at 72 the spills cost more than the seventh brings (64 alone).
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
 __global__ void __launch_bounds__(128, 6) norm_rotary_fwd_kernel(const __grid_constant__ NormParams p) {
   const int lane = threadIdx.x & 31, s = lane % LPR, sub = lane / LPR;
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(128, 6) norm_rotary_fwd_kernel(const __grid_co
 // A warp's stream of groups of rows: jobs `first`, `first` + `step`, .. of q or of k, a job being a token and some of its groups of
 // HPG = 32 / LPR heads.  Rows of x and dy are copied to shared memory DEPTH groups ahead, across jobs, a row's LPR lanes
 // copying its chunks of 16 bytes side by side whatever order they are read in (slots of 32 bytes, a chunk of each at a time, ask L2 for
-// every sector twice: neighbouring pairs 140 us instead of 91).  The angles of a job's token go to a ring
+// every sector twice: neighbouring pairs 140 us instead of 88).  The angles of a job's token go to a ring
 // of their own, copied by one row's lanes for all.  (A group read in this step, DEPTH ahead of it, and the angles of the job behind:
 // DEPTH + 2 entries where every job is one group.)
 // CTAs of 256 threads are resident on an SM as registers (128) and shared memory allow: two, with rows of 32 lanes one, and
@@ -308,7 +309,8 @@ __device__ __forceinline__ void read_angles(f2 (&c)[4], f2 (&sn)[4], uint32_t at
 }
 
 // Backward.  Warps walk q's jobs and then k's with a stride of the grid and keep the sums of dw of their slots in registers.
-// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 82 us, 6.1 TB/s (4 x 4096, 16 / 4 heads, d = 64, 126 MB: 34 us); with the next group's rows in registers 110 us.
+// 2 x 8192 tokens, 32 / 8 heads, d = 128, bf16 (503 MB) in 87 us with the sum of the CTAs' dw, 5.8 TB/s (4 x 4096, 16 / 4 heads, d = 64, 126 MB: 39 us); with
+// the next group's rows in registers 110 us.
 template <bool IS_BF16, bool INTERLEAVED, int LPR>
 __global__ void __launch_bounds__(256, norm_bwd_ctas(LPR)) norm_rotary_bwd_kernel(const __grid_constant__ NormParams p) {
   using Stream = NormStream<LPR>;

@@ -263,12 +263,16 @@ std::pair<Tensor, Tensor> kv_read(const Tensor& ck, const Tensor& cv, const Tens
 
 // Rows (queries x heads of a group) up to which the cache is read by the kernel for few rows.  Beyond, the tokens are
 // read back once into dense 16-bit tensors and the dense forward, which feeds the tensor cores, takes the call.  Measured, 32 / 8
-// heads, d = 128: 96 rows 41 us and 100 rows 50 us for 16384 keys, 70 and 77 us for 8 x 4096, 111 and 98 us for 64 x 512: the
+// heads, d = 128: 96 rows 40 us and 100 rows 52 us for 16384 keys, 69 and 80 us for 8 x 4096, 111 and 102 us for 64 x 512: the
 // kernel's time goes with the number of 32-row tiles and the other's hardly with the rows.
 // Head dims above 128: the dense forward does not deal a row block's K tiles to several CTAs, so its time does not depend on
-// the rows while these leave SMs idle, and the kernel's goes with all rows of the call.  Kernel and dense forward, us: 16384 keys, 32 / 8 heads,
-// d = 192: 112 rows 54 and 277, 640 rows 243 and 372; 4 x 4096: 160 rows 73 and 97; 16384 keys, 16 / 4 heads, d = 256: 112 rows 87 and
-// 185, 224 rows 164 and 185.
+// the rows while these leave SMs idle, and the kernel's goes with all rows of the call: the line is a number of rows of all kv heads together.  Kernel / dense
+// forward, us with the launch (rows of each kv head):
+//   d = 192 (5400)  1 head, 5200 rows of 2048 keys 51 / 63, of 16384 258 / 320, of 65536 942 / 1200;  2 heads, 2000 of 16384 201 / 332, past the line 4000 387 / 330;
+//                   8 heads, 400 of 2048 37 / 57, of 16384 166 / 293, past 1000 of 2048 72 / 72, of 16384 387 / 389;  4 x 8 heads, 168 of 2048 55 / 65, past 400 104 / 65
+//   d = 256 (900)   1 head, 900 of 2048 37 / 49, of 16384 172 / 186, past 1200 223 / 184;  4 heads, 224 of 2048 37 / 47, of 16384 172 / 195, past 480 346 / 197;
+//                   8 heads, 100 of 2048 37 / 49, of 16384 162 / 215, past 224 328 / 215;  4 x 8 heads, past 128 of 2048 117 / 92
+// A window shortens both sides: 1024 of 16384 keys, d = 192, 1 head, 5200 rows 59 / 53, 8 heads, 660 41 / 57, d = 256, 1 head, 896 31 / 43; window 64 43 / 39, 25 / 37, 20 / 35.
 int64_t few_rows(int64_t d, int64_t kv_heads) { return std::max<int64_t>(96, d <= 128 ? 0 : (d <= 192 ? 5400 : 900) / std::max<int64_t>(kv_heads, 1)); }
 // Without an upper bound of the lengths the dense tensors cover the whole page table, which may be far wider than the
 // sequences are long: beyond this many bytes the kernel for few rows, which needs none, keeps the call.

@@ -501,7 +501,8 @@ FM_API int64_t fm_kv_locate(const fm_kv_cache* cache, const fm_kv_args* args, in
 FM_API int fm_kv_write(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
 
 /* k_out [B, S, Hkv, d], v_out [B, S, Hkv, dv] (contiguous): the tokens at positions start[b] + i, zeros where the
- * position is below 0, at seqlens[b] or beyond, or no token.  Exact in bf16; fp16 saturates at 65504.  With `marks` what
+ * position is below 0, at seqlens[b] or beyond, or no token.  Exact in bf16; fp16 saturates at 65504 and
+ * rounds what is below 2^-14 to multiples of 2^-24.  With `marks` what
  * is NaN comes as 0, and marks[b, h] is set where there was some. */
 FM_API int fm_kv_read(const fm_kv_cache* cache, const fm_kv_args* args, void* stream);
 
@@ -516,7 +517,9 @@ FM_API int fm_kv_attention(const fm_kv_cache* cache, const fm_kv_args* args, voi
 
 /* For attention with many query rows over tokens read back into dense tensors of `cols` >= S columns: the position of
  * column 0 of every sequence (`shift` [B], the start of an fm_kv_read of `cols` rows) and the column bounds
- * [B, 1, cols, 1 (causal) | 2] with which fm_fwd sees what fm_kv_attention sees.  With `marks` those are zeroed. */
+ * [B, 1, cols, 1 (causal) | 2] with which fm_fwd sees what fm_kv_attention sees.  The results differ by their roundings: p is fp16
+ * in fm_kv_attention and of q's type in fm_fwd, which gets the tokens as fm_kv_read rounds them.  With a window `cols` need be
+ * no more than S + window - 1.  With `marks` those are zeroed. */
 FM_API int fm_kv_bounds(const fm_kv_cache* cache, const fm_kv_args* args, int cols, int32_t* shift, int32_t* bounds,
                         void* stream);
 
