@@ -341,4 +341,12 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// LSE of a row: m its largest score in log2 units (-inf: it sees nothing), l the sum of exp2(score - m) and l_tot that with the
+// sink's.  The sink is all there is where the row sees nothing (whose sum, against m = 0, may have vanished), or nothing within
+// 2^127 of it (whose sum has overflowed; the row's O is then 0).
+__device__ __forceinline__ float row_lse(const float* sink, int head, float m, float l, float l_tot) {
+  if (sink && ((m == -INFINITY && l == 0.f) || l_tot == INFINITY)) return sink[head];
+  return l_tot > 0.f ? ((m == -INFINITY ? 0.f : m) + log2f(l_tot)) * kLn2 : -INFINITY;
+}
+
 }  // namespace fm

@@ -244,11 +244,12 @@ fwd_mma_kernel(const AttnKParams p) {
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const float m_fin = (m_i[r] == -INFINITY) ? 0.f : m_i[r];
+    const float seen = l;
     if (p.sink) l += fast_exp2(sink_log2 - m_fin);
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const int row = ms + wr * 16 + g + r * 8;
     if (ws == 0 && tq == 0 && row < p.Sq)
-      p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = l > 0.f ? (m_fin + log2f(l)) * kLn2 : -INFINITY;
+      p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = row_lse(p.sink, hq, m_i[r], seen, l);
     const int lrow = wr * 16 + g + r * 8;
 #pragma unroll
     for (int i = 0; i < NT_O; ++i) {

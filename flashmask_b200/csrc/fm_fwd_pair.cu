@@ -408,7 +408,8 @@ fwd_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     ok = group_all(ok, 1, 256);
     if (ok) {
       const float m_fin = (m_run == ninf) ? 0.f : m_run;
-      float l_tot = ex[r] + ex[128 + r];               // fixed order: the same value in both warpgroups
+      const float seen = ex[r] + ex[128 + r];          // fixed order: the same value in both warpgroups
+      float l_tot = seen;
       if (p.sink) l_tot += fast_exp2(p.sink[hq] * kLog2e - m_fin);
       const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
       uint8_t* stage = smem + Cfg::OFF_Q;              // Q is no longer needed; 512-byte rows
@@ -429,7 +430,7 @@ fwd_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       if (slice == 0 && w == 0 && row < p.Sq)
-        p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = l_tot > 0.f ? (m_fin + log2f(l_tot)) * kLn2 : ninf;
+        p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = row_lse(p.sink, hq, m_run, seen, l_tot);
       __syncwarp();   // each warp stores the 32 rows x 128 columns it staged itself
       uint16_t* go = reinterpret_cast<uint16_t*>(p.o) + b * p.o_b + hq * p.o_h + 256 * slice;
       const int wrow = (warp & 3) * 32;

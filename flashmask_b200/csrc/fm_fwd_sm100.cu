@@ -426,7 +426,7 @@ fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           }
         }
         if (prow < n_rows && !(SPLITV && s == 1))
-          p.lse[((int64_t)b * p.Hq + head) * p.Sq + row] = l_tot > 0.f ? (m_fin + log2f(l_tot)) * kLn2 : neg_inf();
+          p.lse[((int64_t)b * p.Hq + head) * p.Sq + row] = row_lse(p.sink, head, m_run, l_run, l_tot);
         __syncwarp();   // each warp stores the 32 rows it staged itself: no cross-warp dependency
         const int rbase = ms + (SPLITV ? 0 : 128 * s);
         uint16_t* go = reinterpret_cast<uint16_t*>(p.o) + b * p.o_b + hq * p.o_h;
@@ -632,6 +632,7 @@ __global__ void __launch_bounds__(256) fwd_combine_kernel(const AttnKParams p) {
   float m = mine;
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));   // (drops NaN; the weights keep it)
+  const float top = m;
   if (m == neg_inf()) m = 0.f;
   const float w_mine = exp2f(mine - m);
   float l = w_mine;
@@ -652,9 +653,10 @@ __global__ void __launch_bounds__(256) fwd_combine_kernel(const AttnKParams p) {
       acc[0] += w * v.x; acc[1] += w * v.y;
     }
   }
+  const float seen = l;
   if (p.sink) l += exp2f(p.sink[h] * kLog2e - m);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  if (lane == 0) p.lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : neg_inf();
+  const float inv = l > 0.f && top != neg_inf() ? 1.f / l : 0.f;          // (a sink alone may be small enough for an infinite quotient)
+  if (lane == 0) p.lse[row] = row_lse(p.sink, h, top, seen, l);
   if (lane * PER < p.dv_dim) {
     uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.o) + b * p.o_b + (int64_t)i * p.o_s + h * p.o_h + lane * PER);
 #pragma unroll

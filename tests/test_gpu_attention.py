@@ -1113,3 +1113,23 @@ def test_overlapping_kernels_of_a_call_replay_from_a_cuda_graph(Sq, Sk, kind):
         for a, b in zip(got, call(*ins)):
             assert torch.equal(a, b)
     assert _kernel_status() == 0
+
+
+@pytest.mark.parametrize("Sq,Sk,Hq,Hkv,d,dv", [(300, 200, 4, 2, 64, 64), (40, 3000, 8, 2, 128, 128), (700, 700, 2, 2, 96, 96), (300, 260, 2, 1, 192, 128),
+                                               (600, 500, 2, 1, 256, 256), (100, 90, 2, 1, 576, 512)])
+def test_sinks_far_from_every_score(Sq, Sk, Hq, Hkv, d, dv):
+    """Sinks 2^127 above the scores and more, and sinks far below beside rows that see nothing: the LSE is the sink then, and gradients are finite."""
+    g = torch.Generator().manual_seed(71)
+    q, k = (torch.randn(2, s, h, d, generator=g).bfloat16().cuda().requires_grad_(True) for s, h in ((Sq, Hq), (Sk, Hkv)))
+    v = k[..., :dv] if d == 576 else torch.randn(2, Sk, Hkv, dv, generator=g).bfloat16().cuda().requires_grad_(True)
+    sink = torch.tensor([200.0, -200.0, 120.0, -95.0])[torch.arange(Hq) % 4].cuda().requires_grad_(True)
+    out, lse = fm.flashmask_attention(q, k, v, causal=True, learnable_sink=sink, return_softmax_lse=True)
+    x = torch.einsum("bihd,bjhd->bhij", q.double(), k.double().repeat_interleave(Hq // Hkv, 2)) / d ** 0.5
+    hidden = torch.arange(Sk, device="cuda")[None] > torch.arange(Sq, device="cuda")[:, None] + Sk - Sq
+    x = torch.cat([x.masked_fill(hidden, -float("inf")), sink.double()[None, :, None, None].expand(2, Hq, Sq, 1)], -1)
+    want = torch.logsumexp(x, -1).detach()
+    # a score is off by d + 16 steps of 2^-23 of the sum of its products' magnitudes, below 6 d^0.5; a sum over Sk keys by Sk steps of 2^-24
+    slack = 6 * d ** 0.5 * (d + 16) * 2.0 ** -23 + Sk * 2.0 ** -24 + 2.0 ** -20
+    assert ((lse.double() - want).abs() <= slack + 2.0 ** -21 * want.abs()).all()
+    grads = torch.autograd.grad(out, [t for t in (q, k, v, sink) if t.is_leaf], torch.ones_like(out))
+    assert all(torch.isfinite(t).all() for t in grads)

@@ -51,7 +51,9 @@ def agrees(f, q, pages, *, q_lengths=None, causal=True, window=None, scale=None,
 
     Half a step of p is 2^-11 in fp16 and 2^-8 in bf16; in fp16 it is absolute below 2^-14: 2^-25, when the largest p is 2^7 at
     least (pages) or 1 (dense), of values of at most 448 scales.  A score is off by d + 16 steps of 2^-23 of the sum of its
-    products' magnitudes, a sum over n keys by n steps of 2^-24, and the result is rounded once."""
+    products' magnitudes, a sum over n keys by n steps of 2^-24, and the result is rounded once.  A sink far above the scores makes
+    the denominator up to 2^127, whose reciprocal is flushed to 0 below 2^-126: that takes at most 2^-126 of the row's sum before the
+    division, n weights of at most 2^15 (pages) or 2^8 (dense) of those values, 2^-111 n 448 scales."""
     B, S, Hq, d = q.shape
     got = fm.kv_cache_attention(q.cuda(), f.cache, f.table.cuda(), f.seqlens.cuda(), causal=causal, window_size=window,
                                 q_lengths=None if q_lengths is None else i32(q_lengths), softmax_scale=scale,
@@ -69,6 +71,8 @@ def agrees(f, q, pages, *, q_lengths=None, causal=True, window=None, scale=None,
         assert torch.equal(torch.isnan(lse[b]), dead.T), b
         slack = reach * (d + 16) * 2.0 ** -23 + 2.0 ** -20 + max(n, 1) * 2.0 ** -24
         tol = half * o.abs() + n * p_least * 448 * f.largest_scale(b) + weight * (p_half + 2 * slack[..., None]) + torch.finfo(q.dtype).smallest_normal * half
+        if sink is not None:
+            tol = tol + n * 2.0 ** -111 * 448 * f.largest_scale(b)
         far = ((out[b] - o).abs() - tol).nan_to_num(nan=-1.0)
         w = far.argmax()
         assert far.flatten()[w] <= 0, (b, int(w), *(t.flatten()[w].item() for t in (far, out[b], o, weight)))
@@ -279,3 +283,14 @@ def test_caches_that_want_a_gradient_are_refused():
             with torch.no_grad():
                 call()
         getattr(f.cache, name).requires_grad_(False)
+
+
+@pytest.mark.parametrize("S,G,d,dv,dtype,pages", [(5, 4, 128, 128, BF16, True), (40, 4, 64, 64, FP16, False), (140, 1, 128, 128, BF16, False), (300, 3, 128, 128, BF16, False),
+                                                  (240, 4, 192, 128, BF16, False), (60, 4, 256, 256, BF16, False), (300, 4, 256, 256, FP16, False)])
+@pytest.mark.parametrize("scale", [None, -0.1])
+def test_sinks_far_from_every_score(S, G, d, dv, dtype, pages, scale):
+    """A sink that is all there is to a row, its scores 2^127 below it and more, and one that is small beside nothing: rows that see nothing."""
+    f = Filled([2000, 300, 0, 20], 2, d, dv, E4M3, 64, seed=52, dtype=dtype)
+    sink = torch.tensor([200.0, -200.0, 0.5, -95.0, 95.0, -1e4])[torch.arange(2 * G) % 6]
+    out, lse = agrees(f, rand_q(4, S, 2 * G, d, seed=53, dtype=dtype), pages, sink=sink, scale=scale, q_lengths=[S, S // 2, S, S])
+    assert torch.equal(lse[2], sink[:, None].expand(2 * G, S).cuda())
