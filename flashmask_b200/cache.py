@@ -97,7 +97,7 @@ def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, page_table:
     are read as they are, and neither ``seqlens`` nor anything else is needed on the host, so the call can be captured into a CUDA graph
     with lengths that change between replays.  With more rows the tokens are read back into 16-bit tensors of ``max_seqlen`` positions
     (an upper bound of ``seqlens``; without it the
-    whole page table, as long as that takes no more than 2 GiB), with a window no more than its last S + ``window_size`` - 1, and go through the dense forward; more positions than it takes (262144 at
+    whole page table, as long as that takes no more than 2 GiB: the call's time goes with these positions, tokens or not), with a window no more than its last S + ``window_size`` - 1, and go through the dense forward; more positions than it takes (262144 at
     head dims other than 256) stay with the pages.  At most 1024 sequences where the pages are read as they are.
 
     Precision: sums and statistics are fp32.  Where the pages are read as they are, the weights p are rounded to fp16 (half a step is 2^-11) whatever query's

@@ -294,3 +294,26 @@ def test_sinks_far_from_every_score(S, G, d, dv, dtype, pages, scale):
     sink = torch.tensor([200.0, -200.0, 0.5, -95.0, 95.0, -1e4])[torch.arange(2 * G) % 6]
     out, lse = agrees(f, rand_q(4, S, 2 * G, d, seed=53, dtype=dtype), pages, sink=sink, scale=scale, q_lengths=[S, S // 2, S, S])
     assert torch.equal(lse[2], sink[:, None].expand(2 * G, S).cuda())
+
+
+def test_a_captured_chunk_sees_what_the_cache_holds_at_a_replay():
+    """NaN that comes and goes between replays, and lengths that change: every replay gives the bits of an eager call."""
+    f = Filled([300, 170], 2, 64, 64, E4M3, 16, seed=54)
+    q, table, n = rand_q(2, 40, 8, 64, seed=55).cuda(), f.table.cuda(), f.seqlens.cuda()
+    clean = f.cache.v.view(torch.uint8).clone()
+    call = lambda: fm.kv_cache_attention(q, f.cache, table, n, max_seqlen=300, return_lse=True)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for pos, lens in ((280, [300, 170]), (None, [300, 170]), (130, [290, 120]), (130, [290, 160])):
+        f.cache.v.view(torch.uint8).copy_(clean)
+        n.copy_(torch.tensor(lens))
+        if pos is not None:
+            for b in range(2):
+                f.cache.v.view(torch.uint8)[page_at(f, b, min(pos, 160)), 1, pos % 16, 3] = 0x7f
+        graph.replay()
+        for a, b in zip(got, call()):
+            assert torch.equal(a.nan_to_num(nan=77.0), b.nan_to_num(nan=77.0))
+        assert bool(torch.isnan(got[0]).any()) == (pos is not None)
